@@ -108,7 +108,7 @@ PTO_API int pto_worker_scratch(pto_worker* w, size_t min_bytes, uint64_t* dev_pt
 /* Registered callables (replaces Worker.register / Worker.run with a ChipCallable:
  * device_runner.py:651-656, worker.py:532-626).  `op_name` names a fused operator:
  * "paged_attention", "paged_gather", "rms_norm", "ffn_swiglu", "linear", "rope_kv_append", "scope3",
- * "decoder_layer", "matmul_mx" (pto_op_list; tensor and scalar order beside each adapter in csrc/ops.cpp and
+ * "decoder_layer", "matmul_mx", "add_rms_norm", "linear_fp8", "swiglu_quantize", "moe_route" (pto_op_list; tensor and scalar order beside each adapter in csrc/ops.cpp and
  * csrc/layer_ops.cpp). */
 PTO_API int pto_register_callable(pto_worker* w, const char* op_name, int32_t* cid);
 PTO_API int pto_unregister_callable(pto_worker* w, int32_t cid);
@@ -210,6 +210,16 @@ PTO_API int pto_cast_zero(const void* in, int in_dtype, void* out, int out_dtype
 PTO_API int pto_linear(const void* x, const void* w_packed, void* out, int m, int n, int k, int accumulate,
                        int32_t* err, void* stream);
 
+/* FP8 linear layer with block scales: out[m, n] = (acc[m, n] +) x @ W over e4m3 operands.
+ *   x e4m3 [m, k] with x_scale fp32 [m, ceil(k / 128)] (pto_quantize_rows, pto_add_rms_norm, pto_swiglu_quantize)
+ *   w e4m3 [n, k] (K contiguous) with w_scale fp32 [ceil(n / 128), ceil(k / 128)], one per 128 x 128 block
+ *   acc fp32 [m, n] or NULL, added to the product (the residual stream); may be out itself when out is fp32
+ *   out bf16 or fp32 [m, n]; fp32 products and sums, rounded once; equal calls give equal bits
+ * The dense counterpart of pto_moe_expert_gemm.  Any m (0: nothing happens), n and k.  Tensor cores run it when k is a
+ * multiple of 16 and x and w are 16-byte aligned; other calls take a slow kernel.  `err` as in pto_linear. */
+PTO_API int pto_linear_fp8(const void* x, const float* x_scale, const void* w, const float* w_scale, const float* acc,
+                           void* out, int out_dtype, int m, int n, int k, int32_t* err, void* stream);
+
 /* Fused SwiGLU FFN: out[m, n_out] (+)= bf16(silu(x Wg) * (x Wu)) Wd.  Replaces `ffn_swiglu`
  * (examples/models/01_ffn.py:112-131) and `mlp_block` + `down_projection_residual`
  * (examples/models/qwen3_jit/kernels/mlp.py:23-61, kernels/projection.py:146-177).
@@ -256,6 +266,18 @@ PTO_API int pto_rms_norm(const void* x, int x_dtype, const float* gamma, void* o
 PTO_API int pto_rms_norm_ex(const void* x, int x_dtype, const float* gamma, void* out, int out_dtype, int64_t rows,
                             int hidden, float eps, float* copy_f32, void* zero, size_t zero_bytes, void* stream);
 
+/* Residual addition and RMSNorm in one pass over the rows, with an optional 8-bit output:
+ *   h = x + residual (fp32; residual NULL: h = x);  y = h * rsqrt(mean(h^2) + eps) * gamma
+ *   x bf16 or fp32 [rows, hidden]; residual and residual_out of one dtype, bf16 or fp32 [rows, hidden];
+ *   residual_out (or NULL) receives h and may be `residual` itself; gamma fp32 [hidden] or NULL
+ *   out (or NULL) receives y in out_dtype; q / scale (both or neither) receive y as FP8 rows: e4m3
+ *   [rows, hidden] with scale fp32 [rows, ceil(hidden / 128)] = max |y| / 448 over 128 columns (1 where that is 0),
+ *   the operands of pto_linear_fp8 and pto_moe_expert_gemm.  One of out and q at least.  hidden up to 49152.
+ * The addition of examples/models/qwen3_jit/kernels/projection.py:146-177 with the norm of kernels/rmsnorm.py:27-89. */
+PTO_API int pto_add_rms_norm(const void* x, int x_dtype, const void* residual, void* residual_out, int res_dtype,
+                             const float* gamma, void* out, int out_dtype, void* q, float* scale, int64_t rows,
+                             int hidden, float eps, void* stream);
+
 /* RoPE (rotate-half) on Q and K at pos = seq_len - 1 and append of the rotated K row and the
  * V row to the paged cache (examples/models/qwen3_jit/kernels/attention.py:40-111).
  *   qkv fp32 [batch, (num_heads + 2*kv_heads) * head_dim]: q heads, k heads, v heads;
@@ -269,6 +291,12 @@ PTO_API int pto_rope_kv_append(const float* qkv, const int32_t* seq_lens, const 
 
 /* act[r, c] = bf16(silu(gate_up[r, c]) * gate_up[r, inter + c]), gate_up fp32 [rows, 2*inter]. */
 PTO_API int pto_swiglu_act(const float* gate_up, void* act, int64_t rows, int inter, void* stream);
+
+/* act[r, c] = silu(gate_up[r, c]) * gate_up[r, inter + c], gate_up bf16 or fp32 [rows, 2*inter], written as FP8 rows:
+ * q e4m3 [rows, inter], scale fp32 [rows, ceil(inter / 128)] as in pto_quantize_rows (from the fp32 activation: no
+ * bf16 rounding in between). */
+PTO_API int pto_swiglu_quantize(const void* gate_up, int dtype, void* q, float* scale, int64_t rows, int inter,
+                                void* stream);
 
 /* ---- tracing (the reference's run-time diagnostics: RunConfig.enable_chip_swimlane and friends,
  * python/pypto/runtime/runner.py:344-348, docs/en/dev/03-runtime-dfx.md:10-18) ----
@@ -298,6 +326,21 @@ PTO_API int pto_llama_mini(const float* hidden, const float* causal_mask, const 
  * indices (sort32 + mrgsort + gather, tests/st/runtime/ops/test_sort.py:602-632): exact integers. */
 PTO_API int pto_moe_topk(const float* scores, const float* bias, int is_logits, int tokens, int experts,
                          int topk, int32_t* idx, float* weights, void* stream);
+
+/* Routing with score functions and expert groups:
+ *   score = sigmoid(logit) (PTO_SCORE_SIGMOID) or softmax over the experts (PTO_SCORE_SOFTMAX); key = score + bias
+ *   (bias fp32 [experts] or NULL); the experts form n_group groups of neighbours, a group's score is the sum of its
+ *   best group_top (1 or 2) keys, the best topk_group groups stay; idx int32 [tokens, topk] = the topk experts by key
+ *   among them, descending; weights fp32 [tokens, topk] = their scores (not keys), divided by their sum if renormalize,
+ *   times route_scale.  logits fp32 or bf16 [tokens, experts].
+ * Ties go to the lower id; keys and group scores compare as they are in 64 bits.  A bias of -inf takes an expert out, a
+ * NaN key does too; rows without enough experts left are filled with the lowest unused ids at weight 0.
+ * At most 1024 experts, topk up to 32 and up to the experts of topk_group groups.  n_group = topk_group = 1 for a
+ * router without groups. */
+enum { PTO_SCORE_SIGMOID = 0, PTO_SCORE_SOFTMAX = 1 };
+PTO_API int pto_moe_route(const void* logits, int logits_dtype, const float* bias, int scoring, int tokens, int experts,
+                          int n_group, int topk_group, int group_top, int topk, int renormalize, float route_scale,
+                          int32_t* idx, float* weights, void* stream);
 
 /* Per-(row, 128 columns) e4m3 quantisation: scale = amax / 448 (1 for an all-zero group),
  * q = e4m3(x / scale) round-to-nearest-even.  x bf16 or fp32 [rows, cols], cols % 128 == 0. */
@@ -470,6 +513,10 @@ PTO_API int pto_moe_layer_peer_exchange(const pto_moe_layer* layer); /* 0: colle
 PTO_API int pto_moe_layer_forward(pto_moe_layer* layer, const void* x, int tokens, const int32_t* idx_in,
                                   const float* w_in, void* y, int32_t* idx_out, float* w_out, float* phase_ms,
                                   void* stream);
+/* How the layer routes from its next forward call on: pto_moe_route over the gate's logits with the layer's bias,
+ * instead of the default (pto_moe_topk: sigmoid, no groups, weights that sum to one).  On every rank alike. */
+PTO_API int pto_moe_layer_set_router(pto_moe_layer* layer, int scoring, int n_group, int topk_group, int group_top,
+                                     int renormalize, float route_scale);
 /* Reads (and clears) the layer's device error word, see pto_device_status; synchronises `stream`. */
 PTO_API int pto_moe_layer_status(pto_moe_layer* layer, int32_t out[4], void* stream);
 

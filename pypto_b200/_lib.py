@@ -83,6 +83,10 @@ SIGNATURES = {
     "pto_set_trace": (_i, [_i]),
     "pto_get_trace": (_i, []),
     "pto_last_run_ms": (_i, [_p, C.POINTER(C.c_float)]),
+    "pto_add_rms_norm": (_i, [_p, _i, _p, _p, _i, _p, _p, _i, _p, _p, _i64, _i, _f, _p]),
+    "pto_swiglu_quantize": (_i, [_p, _i, _p, _p, _i64, _i, _p]),
+    "pto_linear_fp8": (_i, [_p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _p, _p]),
+    "pto_moe_route": (_i, [_p, _i, _p, _i, _i, _i, _i, _i, _i, _i, _i, _f, _p, _p, _p]),
     "pto_moe_topk": (_i, [_p, _p, _i, _i, _i, _i, _p, _p, _p]),
     "pto_quantize_rows": (_i, [_p, _i, _p, _p, _i64, _i, _p]),
     "pto_moe_dispatch_plan": (_i, [_p, _i, _i, _p, _p, _p, _p, _p, _p, _p]),
@@ -120,6 +124,7 @@ SIGNATURES.update({
     "pto_moe_layer_create": (_i, [C.POINTER(MoeLayerDesc), C.POINTER(_p)]),
     "pto_moe_layer_destroy": (_i, [_p]),
     "pto_moe_layer_forward": (_i, [_p, _p, _i, _p, _p, _p, _p, _p, C.POINTER(C.c_float), _p]),
+    "pto_moe_layer_set_router": (_i, [_p, _i, _i, _i, _i, _i, _f]),
     "pto_moe_layer_status": (_i, [_p, _i32p, _p]),
     "pto_moe_layer_peer_exchange": (_i, [_p]),
 })

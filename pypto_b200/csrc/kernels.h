@@ -85,6 +85,22 @@ int cast_zero_launch(const void* in, int in_dtype, void* out, int out_dtype, lon
                      size_t zero_bytes, cudaStream_t stream);
 int pack_weight_launch(const void* src, int src_dtype, void* dst, int k, int n, cudaStream_t stream);
 
+// fp8_rows.cu
+int add_rms_norm_launch(const void* x, int x_dtype, const void* residual, void* residual_out, int res_dtype,
+                        const float* gamma, void* out, int out_dtype, void* q, float* scale, long long rows, int hidden,
+                        float eps, cudaStream_t stream);
+int swiglu_quantize_launch(const void* gate_up, int dtype, void* q, float* scale, long long rows, int inter,
+                           cudaStream_t stream);
+
+// linear_fp8.cu
+int linear_fp8_launch(const void* x, const float* x_scale, const void* w, const float* w_scale, const float* acc, void* out,
+                      int out_dtype, int m, int n, int k, int* err, cudaStream_t stream);
+
+// moe_select.cu
+int moe_route_launch(const void* logits, int logits_dtype, const float* bias, int scoring, int tokens, int experts,
+                     int n_group, int topk_group, int group_top, int topk, int renormalize, float route_scale,
+                     int32_t* idx, float* weights, cudaStream_t stream);
+
 // moe_route.cu
 int moe_topk_launch(const float* scores, const float* bias, int is_logits, int tokens, int experts, int topk,
                     int32_t* idx, float* weights, cudaStream_t stream);

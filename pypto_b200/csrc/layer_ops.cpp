@@ -354,4 +354,85 @@ int op_llama_mini(Worker* w, const pto_task_args* a) {
                            static_cast<float*>(tptr(t[12], 4)), s, d, v, w->stream);
 }
 
+// tensors: x [rows, hidden] (bf16 or fp32), residual [rows, hidden] (bf16 or fp32; updated in place), gamma fp32 [hidden],
+//          out [rows, hidden] (bf16 or fp32), or e4m3 q [rows, hidden] and scale fp32 [rows, ceil(hidden / 128)] in
+//          its place
+// scalars: eps (fp32 bits)
+int op_add_rms_norm(Worker* w, const pto_task_args* a) {
+  if ((a->n_tensors != 4 && a->n_tensors != 5) || a->n_scalars != 1)
+    return fail(kInvalidArgument, "add_rms_norm: expects 4 tensors (or 5: q and scale instead of out) and 1 scalar");
+  const pto_chip_tensor* t = a->tensors;
+  if (t[0].ndims != 2) return fail(kInvalidArgument, "add_rms_norm: x [rows, hidden] expected");
+  const int rows = t[0].shapes[0], hidden = t[0].shapes[1];
+  const bool quant = a->n_tensors == 5;
+  auto wide = [](const pto_chip_tensor& v) { return v.dtype == PTO_BF16 || v.dtype == PTO_FP32; };
+  bool ok = wide(t[0]) && wide(t[1]) && numel(t[1]) == numel(t[0]) && t[2].dtype == PTO_FP32 && numel(t[2]) == hidden &&
+            numel(t[3]) == numel(t[0]) && (quant ? t[3].dtype == PTO_FP8E4M3 : wide(t[3]));
+  if (quant) ok = ok && is2d(t[4], rows, (hidden + 127) / 128, PTO_FP32);
+  if (!ok) return fail(kInvalidArgument, "add_rms_norm: tensor shapes or dtypes do not match");
+  void* res = tptr(t[1], t[1].dtype == PTO_BF16 ? 2 : 4);
+  uint32_t bits = static_cast<uint32_t>(a->scalars[0]);
+  float eps;
+  memcpy(&eps, &bits, 4);
+  return add_rms_norm_launch(tptr(t[0], t[0].dtype == PTO_BF16 ? 2 : 4), (int)t[0].dtype, res, res, (int)t[1].dtype,
+                             static_cast<const float*>(tptr(t[2], 4)),
+                             quant ? nullptr : tptr(t[3], t[3].dtype == PTO_BF16 ? 2 : 4), quant ? PTO_BF16 : (int)t[3].dtype,
+                             quant ? tptr(t[3], 1) : nullptr, quant ? static_cast<float*>(tptr(t[4], 4)) : nullptr, rows,
+                             hidden, eps, w->stream);
+}
+
+// tensors: x e4m3 [m, k], x_scale fp32 [m, ceil(k / 128)], w e4m3 [n, k], w_scale fp32 [ceil(n / 128), ceil(k / 128)],
+//          out [m, n] (bf16 or fp32), optionally acc fp32 [m, n]
+int op_linear_fp8(Worker* w, const pto_task_args* a) {
+  if ((a->n_tensors != 5 && a->n_tensors != 6) || a->n_scalars != 0)
+    return fail(kInvalidArgument, "linear_fp8: expects 5 or 6 tensors and no scalars");
+  const pto_chip_tensor* t = a->tensors;
+  if (t[0].ndims != 2 || t[2].ndims != 2) return fail(kInvalidArgument, "linear_fp8: x [m, k] and w [n, k] expected");
+  const int m = t[0].shapes[0], k = t[0].shapes[1], n = t[2].shapes[0], kb = (k + 127) / 128;
+  const bool ok = t[0].dtype == PTO_FP8E4M3 && t[2].dtype == PTO_FP8E4M3 && (int)t[2].shapes[1] == k &&
+                  is2d(t[1], m, kb, PTO_FP32) && is2d(t[3], (n + 127) / 128, kb, PTO_FP32) &&
+                  (is2d(t[4], m, n, PTO_BF16) || is2d(t[4], m, n, PTO_FP32)) &&
+                  (a->n_tensors == 5 || is2d(t[5], m, n, PTO_FP32));
+  if (!ok) return fail(kInvalidArgument, "linear_fp8: tensor shapes or dtypes do not match");
+  int st = w->ensure_scratch(256);
+  if (st != kOk) return st;
+  return linear_fp8_launch(tptr(t[0], 1), static_cast<const float*>(tptr(t[1], 4)), tptr(t[2], 1),
+                           static_cast<const float*>(tptr(t[3], 4)),
+                           a->n_tensors == 6 ? static_cast<const float*>(tptr(t[5], 4)) : nullptr,
+                           tptr(t[4], t[4].dtype == PTO_BF16 ? 2 : 4), (int)t[4].dtype, m, n, k,
+                           static_cast<int*>(w->scratch), w->stream);
+}
+
+// tensors: gate_up [rows, 2 * inter] (bf16 or fp32), q e4m3 [rows, inter], scale fp32 [rows, ceil(inter / 128)]
+int op_swiglu_quantize(Worker* w, const pto_task_args* a) {
+  if (a->n_tensors != 3 || a->n_scalars != 0) return fail(kInvalidArgument, "swiglu_quantize: expects 3 tensors");
+  const pto_chip_tensor* t = a->tensors;
+  if (t[0].ndims != 2 || t[0].shapes[1] % 2 || (t[0].dtype != PTO_BF16 && t[0].dtype != PTO_FP32))
+    return fail(kInvalidArgument, "swiglu_quantize: gate_up bf16 or fp32 [rows, 2 * inter] expected");
+  const int rows = t[0].shapes[0], inter = t[0].shapes[1] / 2;
+  if (!is2d(t[1], rows, inter, PTO_FP8E4M3) || !is2d(t[2], rows, (inter + 127) / 128, PTO_FP32))
+    return fail(kInvalidArgument, "swiglu_quantize: q or scale does not match");
+  return swiglu_quantize_launch(tptr(t[0], t[0].dtype == PTO_BF16 ? 2 : 4), (int)t[0].dtype, tptr(t[1], 1),
+                                static_cast<float*>(tptr(t[2], 4)), rows, inter, w->stream);
+}
+
+// tensors: logits [tokens, experts] (fp32 or bf16), bias fp32 [experts], idx int32 [tokens, topk], weights fp32 [tokens, topk]
+// scalars: scoring, n_group, topk_group, group_top, renormalize, route_scale (fp32 bits)
+int op_moe_route(Worker* w, const pto_task_args* a) {
+  if (a->n_tensors != 4 || a->n_scalars != 6) return fail(kInvalidArgument, "moe_route: expects 4 tensors and 6 scalars");
+  const pto_chip_tensor* t = a->tensors;
+  if (t[0].ndims != 2 || t[2].ndims != 2) return fail(kInvalidArgument, "moe_route: logits [tokens, experts] and idx [tokens, topk] expected");
+  const int tokens = t[0].shapes[0], experts = t[0].shapes[1], topk = t[2].shapes[1];
+  if ((t[0].dtype != PTO_FP32 && t[0].dtype != PTO_BF16) || t[1].dtype != PTO_FP32 || numel(t[1]) != experts ||
+      !is2d(t[2], tokens, topk, PTO_INT32) || !is2d(t[3], tokens, topk, PTO_FP32))
+    return fail(kInvalidArgument, "moe_route: tensor shapes or dtypes do not match");
+  const uint64_t* s = a->scalars;
+  uint32_t bits = static_cast<uint32_t>(s[5]);
+  float scale;
+  memcpy(&scale, &bits, 4);
+  return moe_route_launch(tptr(t[0], t[0].dtype == PTO_BF16 ? 2 : 4), (int)t[0].dtype, static_cast<const float*>(tptr(t[1], 4)),
+                          (int)s[0], tokens, experts, (int)s[1], (int)s[2], (int)s[3], topk, (int)s[4], scale,
+                          static_cast<int32_t*>(tptr(t[2], 4)), static_cast<float*>(tptr(t[3], 4)), w->stream);
+}
+
 }  // namespace pto

@@ -71,6 +71,10 @@ struct pto_moe_layer {
   // peer-memory paths: 1 = the way back, 2 = the way out as well
   bool peer = false;
   int peer_level = 0;
+  // routing: moe_topk until pto_moe_layer_set_router asks for moe_route
+  bool router = false;
+  int scoring = 0, n_group = 1, topk_group = 1, group_top = 1, renormalize = 1;
+  float route_scale = 1.f;
   int step = 0;                     // forward calls so far: the value this rank's flags are raised to
   int32_t *flags = nullptr, *done_counter = nullptr, *base_send = nullptr, *base_recv = nullptr;   // in the arena
   int32_t *flags_out = nullptr, *done_counter_out = nullptr, *obase_send = nullptr, *obase_recv = nullptr;
@@ -268,6 +272,20 @@ int pto_moe_layer_create(const pto_moe_layer_desc* desc, pto_moe_layer** out) {
 
 int pto_moe_layer_peer_exchange(const pto_moe_layer* L) { return L && L->peer ? L->peer_level : 0; }
 
+int pto_moe_layer_set_router(pto_moe_layer* L, int scoring, int n_group, int topk_group, int group_top, int renormalize,
+                             float route_scale) {
+  using namespace pto;
+  if (!L) return fail(kInvalidArgument, "moe_layer_set_router: NULL layer");
+  // a call for no tokens checks the rest
+  const int st = moe_route_launch(nullptr, PTO_FP32, nullptr, scoring, 0, L->d.n_experts, n_group, topk_group, group_top,
+                                  L->d.topk, renormalize, route_scale, nullptr, nullptr, nullptr);
+  if (st != kOk) return st;
+  L->scoring = scoring; L->n_group = n_group; L->topk_group = topk_group; L->group_top = group_top;
+  L->renormalize = renormalize; L->route_scale = route_scale;
+  L->router = true;
+  return kOk;
+}
+
 int pto_moe_layer_status(pto_moe_layer* L, int32_t out4[4], void* stream) {
   using namespace pto;
   if (!L || !out4) return fail(kInvalidArgument, "moe_layer_status: NULL argument");
@@ -314,7 +332,9 @@ int pto_moe_layer_forward(pto_moe_layer* L, const void* x, int tokens, const int
   if (!idx_in) {
     st = linear_launch(x, d.gate_packed, L->logits, T, E, H, 0, L->err, s);
     if (st != kOk) return st;
-    st = moe_topk_launch(L->logits, d.bias, 1, T, E, K, L->idx, L->w, s);
+    st = L->router ? moe_route_launch(L->logits, PTO_FP32, d.bias, L->scoring, T, E, L->n_group, L->topk_group, L->group_top, K,
+                                      L->renormalize, L->route_scale, L->idx, L->w, s)
+                   : moe_topk_launch(L->logits, d.bias, 1, T, E, K, L->idx, L->w, s);
     if (st != kOk) return st;
     idx = L->idx;
     w = L->w;

@@ -200,6 +200,10 @@ const OpEntry kOps[] = {
     {"matmul_mx", op_matmul_mx},
     {"moe_layer", op_moe_layer},
     {"llama_mini", op_llama_mini},
+    {"add_rms_norm", op_add_rms_norm},
+    {"linear_fp8", op_linear_fp8},
+    {"swiglu_quantize", op_swiglu_quantize},
+    {"moe_route", op_moe_route},
 };
 
 }  // namespace
@@ -351,6 +355,30 @@ int pto_llama_mini(const float* hidden, const float* causal_mask, const float* c
 
 int pto_swiglu_act(const float* gate_up, void* act, int64_t rows, int inter, void* stream) {
   return pto::swiglu_act_launch(gate_up, act, rows, inter, static_cast<cudaStream_t>(stream));
+}
+
+int pto_add_rms_norm(const void* x, int x_dtype, const void* residual, void* residual_out, int res_dtype,
+                     const float* gamma, void* out, int out_dtype, void* q, float* scale, int64_t rows, int hidden,
+                     float eps, void* stream) {
+  return pto::add_rms_norm_launch(x, x_dtype, residual, residual_out, res_dtype, gamma, out, out_dtype, q, scale, rows,
+                                  hidden, eps, static_cast<cudaStream_t>(stream));
+}
+
+int pto_swiglu_quantize(const void* gate_up, int dtype, void* q, float* scale, int64_t rows, int inter, void* stream) {
+  return pto::swiglu_quantize_launch(gate_up, dtype, q, scale, rows, inter, static_cast<cudaStream_t>(stream));
+}
+
+int pto_linear_fp8(const void* x, const float* x_scale, const void* w, const float* w_scale, const float* acc, void* out,
+                   int out_dtype, int m, int n, int k, int32_t* err, void* stream) {
+  return pto::linear_fp8_launch(x, x_scale, w, w_scale, acc, out, out_dtype, m, n, k, err,
+                                static_cast<cudaStream_t>(stream));
+}
+
+int pto_moe_route(const void* logits, int logits_dtype, const float* bias, int scoring, int tokens, int experts,
+                  int n_group, int topk_group, int group_top, int topk, int renormalize, float route_scale, int32_t* idx,
+                  float* weights, void* stream) {
+  return pto::moe_route_launch(logits, logits_dtype, bias, scoring, tokens, experts, n_group, topk_group, group_top, topk,
+                               renormalize, route_scale, idx, weights, static_cast<cudaStream_t>(stream));
 }
 
 int pto_moe_topk(const float* scores, const float* bias, int is_logits, int tokens, int experts, int topk,

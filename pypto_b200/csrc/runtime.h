@@ -64,5 +64,9 @@ int op_rope_kv_append(Worker* w, const pto_task_args* a);
 int op_matmul_mx(Worker* w, const pto_task_args* a);
 int op_moe_layer(Worker* w, const pto_task_args* a);
 int op_llama_mini(Worker* w, const pto_task_args* a);
+int op_add_rms_norm(Worker* w, const pto_task_args* a);
+int op_linear_fp8(Worker* w, const pto_task_args* a);
+int op_swiglu_quantize(Worker* w, const pto_task_args* a);
+int op_moe_route(Worker* w, const pto_task_args* a);
 
 }  // namespace pto

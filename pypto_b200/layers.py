@@ -50,6 +50,62 @@ class SwiGLUFFN:
         return (self.w_gate_up.numel() + self.w_down.numel()) * 2
 
 
+def quantize_weight(w: torch.Tensor):
+    """[K, N] float (the ``x @ W`` layout) -> (e4m3 [N, K], scale fp32 [ceil(N/128), ceil(K/128)]), the operand of
+    ``ops.linear_fp8``: scale = max |w| / 448 over a 128 x 128 block (1 where that is 0).  One-time, like pack_weight."""
+    if w.dim() != 2 or not w.is_floating_point():
+        raise TypeError("quantize_weight expects a 2-D floating-point tensor")
+    k, n = w.shape
+    nb, kb = (n + 127) // 128, (k + 127) // 128
+    t = torch.zeros(nb * 128, kb * 128, dtype=torch.float32, device=w.device)
+    t[:n, :k] = w.t()
+    blocks = t.view(nb, 128, kb, 128)
+    scale = blocks.abs().amax(dim=(1, 3)) / 448.0
+    scale = torch.where(scale > 0, scale, torch.ones_like(scale))
+    q = (blocks / scale.view(nb, 1, kb, 1)).view(nb * 128, kb * 128)[:n, :k].to(ops.FP8)
+    return q.contiguous(), scale.contiguous()
+
+
+class Fp8SwiGLUFFN:
+    """The feed-forward block of a decoder layer with FP8 weights and activations, from the residual stream back into
+    it: add + RMSNorm -> gate/up projection -> SwiGLU -> down projection + residual (the block of
+    examples/models/qwen3_jit/kernels/rmsnorm.py:58-89 and kernels/mlp.py:23-61, kernels/projection.py:146-177 in FP8).
+
+    Four launches; between them only FP8 rows and the bf16 gate/up product touch memory."""
+
+    launches_per_call = 4
+
+    def __init__(self, w_gate_up: tuple, w_down: tuple, gamma: torch.Tensor, eps: float):
+        """``w_gate_up`` = (e4m3 [2*inter, hidden], scales) with the gate rows first, ``w_down`` = (e4m3 [hidden, inter],
+        scales), both as ``quantize_weight`` makes them; gamma fp32 [hidden]."""
+        (self.w_gu, self.s_gu), (self.w_d, self.s_d) = w_gate_up, w_down
+        self.gamma, self.eps = gamma.reshape(-1).contiguous(), float(eps)
+        self.hidden, self.inter = self.w_gu.shape[1], self.w_gu.shape[0] // 2
+        if self.w_gu.shape[0] % 2 or tuple(self.w_d.shape) != (self.hidden, self.inter):
+            raise ValueError("Fp8SwiGLUFFN: weights must be [2*inter, hidden] and [hidden, inter]")
+
+    @classmethod
+    def from_float(cls, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, gamma: torch.Tensor, eps: float):
+        """From float weights in the ``x @ W`` layout ([hidden, inter], [hidden, inter], [inter, hidden])."""
+        return cls(quantize_weight(torch.cat([w_gate, w_up], dim=1)), quantize_weight(w_down), gamma, eps)
+
+    def __call__(self, x: torch.Tensor | None, residual: torch.Tensor) -> torch.Tensor:
+        """residual (fp32 [rows, hidden], updated in place) += x; then += FFN(RMSNorm(residual)).  ``x`` is the output of
+        the block before (bf16 or fp32 [rows, hidden]) or None when it is in the residual already."""
+        if residual.dtype != torch.float32 or residual.dim() != 2 or residual.shape[1] != self.hidden:
+            raise ValueError("Fp8SwiGLUFFN: residual must be fp32 [rows, hidden]")
+        if x is None:
+            q, s = ops.add_rms_norm_quantize(residual, None, self.gamma, self.eps)
+        else:
+            q, s = ops.add_rms_norm_quantize(x, residual, self.gamma, self.eps)
+        gate_up = ops.linear_fp8(q, s, self.w_gu, self.s_gu)
+        q, s = ops.swiglu_quantize(gate_up)
+        return ops.linear_fp8(q, s, self.w_d, self.s_d, acc=residual, out=residual)
+
+    def weight_bytes(self) -> int:
+        return self.w_gu.numel() + self.w_d.numel() + 4 * (self.s_gu.numel() + self.s_d.numel())
+
+
 class DecoderLayer:
     # kernels of one step: RMSNorm, QKV GEMM, RoPE + append, attention, merge, O GEMM, RMSNorm, gate/up GEMM,
     # SwiGLU, down GEMM, cast

@@ -22,9 +22,23 @@ local and no collective.
 
 from __future__ import annotations
 
+from dataclasses import dataclass
+
 import torch
 
 from . import ops
+
+
+@dataclass(frozen=True)
+class Router:
+    """How a ``MoELayer`` turns gate logits into experts and weights: the options of ``ops.moe_route``.  A layer built
+    without one routes by sigmoid scores, without groups, with weights that sum to one (``ops.moe_topk``)."""
+    scoring: str = "sigmoid"
+    n_group: int = 1
+    topk_group: int = 1
+    group_top: int = 2
+    renormalize: bool = True
+    route_scale: float = 1.0
 
 
 def pack_expert_weights(stacked: dict) -> dict:
@@ -203,18 +217,19 @@ class PhaseTimer:
 
 class MoELayer:
     def __init__(self, gate_w: torch.Tensor, bias: torch.Tensor, routed: dict, shared: dict | None, topk: int,
-                 n_experts: int | None = None, comm=None):
+                 n_experts: int | None = None, comm=None, router: Router | None = None):
         """gate_w bf16 [H, E_global]; bias fp32 [E_global]; ``routed``: this rank's experts
         (stacked, ``x @ W`` layout, see pack_expert_weights); ``shared``: one expert (no leading
-        dim) or None.  With a communicator, global expert e lives on rank e // L."""
-        self._setup(comm, routed["wg"].shape[0], n_experts, topk)
+        dim) or None.  With a communicator, global expert e lives on rank e // L.  ``router``: scores, groups and
+        weights of the routing (the same on every rank); None keeps the plain sigmoid top-k."""
+        self._setup(comm, routed["wg"].shape[0], n_experts, topk, router)
         self.gate_packed = ops.pack_weight(gate_w.contiguous())
         self.bias = bias.float().contiguous()
         self.routed = pack_expert_weights(routed)
         self.shared = pack_expert_weights({k: v.unsqueeze(0) for k, v in shared.items()}) if shared else None
         self.hidden = gate_w.shape[0]
 
-    def _setup(self, comm, local_experts, n_experts, topk):
+    def _setup(self, comm, local_experts, n_experts, topk, router=None):
         self.comm = comm
         self.world = comm.world if comm is not None else 1
         self.rank = comm.rank if comm is not None else 0
@@ -223,21 +238,29 @@ class MoELayer:
         if self.n_experts != self.local_experts * self.world:
             raise ValueError("experts must be split evenly over the ranks")
         self.topk = topk
+        if router is not None:
+            ops.check_routing(self.n_experts, topk, router.scoring, router.n_group, router.topk_group, router.group_top)
+        self.router = router
         self._handle, self._handle_tokens = None, 0
 
     @classmethod
     def from_packed(cls, gate_packed: torch.Tensor, bias: torch.Tensor, routed: dict, shared: dict | None,
-                    topk: int, n_experts: int | None = None, comm=None) -> "MoELayer":
+                    topk: int, n_experts: int | None = None, comm=None, router: Router | None = None) -> "MoELayer":
         """Build from weights already in the kernels' layout (gate packed [E, H] bf16; expert
         dicts with w_gu / s_gu / w_d / s_d as produced by pack_expert_weights)."""
         self = cls.__new__(cls)
-        self._setup(comm, routed["w_gu"].shape[0], n_experts, topk)
+        self._setup(comm, routed["w_gu"].shape[0], n_experts, topk, router)
         self.gate_packed, self.bias = gate_packed, bias.float().contiguous()
         self.routed, self.shared, self.hidden = routed, shared, gate_packed.shape[1]
         return self
 
     def route(self, x: torch.Tensor):
         logits = ops.linear(x, self.gate_packed)
+        r = self.router
+        if r is not None:
+            return ops.moe_route(logits, self.topk, bias=self.bias, scoring=r.scoring, n_group=r.n_group,
+                                 topk_group=r.topk_group, group_top=r.group_top, renormalize=r.renormalize,
+                                 route_scale=r.route_scale)
         return ops.moe_topk(logits, self.bias, self.topk, is_logits=True)
 
     PHASES = ("route_quantize", "plan", "pack", "exchange_out", "unpack", "experts", "exchange_back", "combine")
@@ -266,6 +289,13 @@ class MoELayer:
         out = C.c_void_p()
         with torch.cuda.device(dev):
             _lib.check(lib.pto_moe_layer_create(C.byref(d), C.byref(out)))
+        r = self.router
+        if r is not None:
+            st = lib.pto_moe_layer_set_router(out, ops.SCORING[r.scoring], r.n_group, r.topk_group, r.group_top,
+                                              1 if r.renormalize else 0, float(r.route_scale))
+            if st != 0:
+                lib.pto_moe_layer_destroy(out)
+            _lib.check(st)
         self._handle, self._handle_tokens = out, tokens
         return out
 

@@ -22,6 +22,8 @@ if hasattr(torch, "float8_e4m3fn"):
 if hasattr(torch, "float8_e8m0fnu"):
     _DT[torch.float8_e8m0fnu] = _lib.PTO_UINT8          # E8M0 scale codes travel as bytes
 
+FP8 = torch.float8_e4m3fn
+
 _scratch: dict[tuple[int, int], torch.Tensor] = {}
 
 
@@ -226,6 +228,40 @@ def linear(x: torch.Tensor, w_packed: torch.Tensor, out: torch.Tensor | None = N
     return out
 
 
+def linear_fp8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, *,
+               acc: torch.Tensor | None = None, out: torch.Tensor | None = None,
+               out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """out[m, n] = (acc +) x @ W with FP8 rows x (e4m3 [m, k], x_scale fp32 [m, ceil(k/128)], as ``quantize_rows`` and
+    its fused forms write them) and a weight w e4m3 [n, k] with one fp32 scale per 128 x 128 block (w_scale
+    [ceil(n/128), ceil(k/128)]).  out bf16 or fp32 (``out_dtype`` when it is not given); acc fp32 [m, n], may be out."""
+    dev = _need_cuda(*[t for t in (x, x_scale, w, w_scale, acc, out) if t is not None])
+    if x.dtype != FP8 or w.dtype != FP8 or x.dim() != 2 or w.dim() != 2:
+        raise TypeError("linear_fp8: x and w must be 2-D float8_e4m3fn tensors")
+    m, k = x.shape
+    n, k2 = w.shape
+    if k != k2 or k < 1 or n < 1:
+        raise ValueError(f"linear_fp8: x has k={k}, w is [{n}, {k2}]")
+    kb = (k + 127) // 128
+    if x_scale.dtype != torch.float32 or w_scale.dtype != torch.float32:
+        raise TypeError("linear_fp8: scales must be fp32")
+    if tuple(x_scale.shape) != (m, kb) or tuple(w_scale.shape) != ((n + 127) // 128, kb):
+        raise ValueError(f"linear_fp8: scales must be [{m}, {kb}] and [{(n + 127) // 128}, {kb}]")
+    if out is None:
+        if out_dtype not in (torch.bfloat16, torch.float32):
+            raise TypeError("linear_fp8: out is bf16 or fp32")
+        out = torch.empty(m, n, dtype=out_dtype, device=dev)
+    elif out.dtype not in (torch.bfloat16, torch.float32) or tuple(out.shape) != (m, n):
+        raise ValueError("linear_fp8: out must be a bf16 or fp32 [m, n] tensor")
+    if acc is not None and (acc.dtype != torch.float32 or tuple(acc.shape) != (m, n)):
+        raise ValueError("linear_fp8: acc must be fp32 [m, n]")
+    with torch.cuda.device(dev):
+        _lib.check(_lib.load().pto_linear_fp8(
+            x.data_ptr(), x_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(),
+            acc.data_ptr() if acc is not None else None, out.data_ptr(), dtype_code(out.dtype), m, n, k, _err_ptr(dev),
+            _stream_ptr(dev)))
+    return out
+
+
 _ffn_ws: dict = {}
 
 
@@ -295,6 +331,56 @@ def rms_norm(x: torch.Tensor, gamma: torch.Tensor | None, eps: float, out_dtype:
     return out
 
 
+def _norm_call(x, residual, gamma, eps, out_dtype, residual_out, quantize: bool, name: str):
+    dev = _need_cuda(*[t for t in (x, residual, gamma, residual_out) if t is not None])
+    if x.dim() < 1 or x.shape[-1] < 1 or x.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"{name}: x must be bf16 or fp32 [..., hidden]")
+    hidden = x.shape[-1]
+    rows = x.numel() // hidden
+    for t, what in ((residual, "residual"), (residual_out, "residual_out")):
+        if t is not None and (t.shape != x.shape or t.dtype not in (torch.bfloat16, torch.float32)):
+            raise ValueError(f"{name}: {what} must be bf16 or fp32 with the shape of x")
+    if residual is not None and residual_out is not None and residual.dtype != residual_out.dtype:
+        raise ValueError(f"{name}: residual and residual_out must have one dtype")
+    if gamma is not None and (gamma.dtype != torch.float32 or gamma.numel() != hidden):
+        raise ValueError(f"{name}: gamma must be fp32 with hidden elements")
+    if out_dtype not in (None, torch.bfloat16, torch.float32):
+        raise TypeError(f"{name}: the normed rows are bf16 or fp32")
+    if residual_out is None:
+        residual_out = residual
+    stored = residual if residual is not None else residual_out
+    out = torch.empty(x.shape, dtype=out_dtype, device=dev) if out_dtype is not None else None
+    q = torch.empty(x.shape, dtype=FP8, device=dev) if quantize else None
+    scale = torch.empty(*x.shape[:-1], (hidden + 127) // 128, dtype=torch.float32, device=dev) if quantize else None
+    with torch.cuda.device(dev):
+        _lib.check(_lib.load().pto_add_rms_norm(
+            x.data_ptr(), dtype_code(x.dtype), residual.data_ptr() if residual is not None else None,
+            residual_out.data_ptr() if residual_out is not None else None,
+            dtype_code(stored.dtype) if stored is not None else _lib.PTO_FP32,
+            gamma.data_ptr() if gamma is not None else None, out.data_ptr() if out is not None else None,
+            dtype_code(out_dtype) if out is not None else _lib.PTO_BF16, q.data_ptr() if quantize else None,
+            scale.data_ptr() if quantize else None, rows, hidden, float(eps), _stream_ptr(dev)))
+    return out, q, scale
+
+
+def add_rms_norm(x: torch.Tensor, residual: torch.Tensor | None, gamma: torch.Tensor | None, eps: float,
+                 out_dtype: torch.dtype = torch.bfloat16, *, residual_out: torch.Tensor | None = None) -> torch.Tensor:
+    """RMSNorm of the rows of x + residual; the sum goes to ``residual_out``, by default into ``residual`` itself
+    (rounded to its dtype; the norm is taken of the fp32 sum).  ``residual`` None: the norm of x."""
+    if out_dtype is None:
+        raise TypeError("add_rms_norm: the normed rows are bf16 or fp32")
+    return _norm_call(x, residual, gamma, eps, out_dtype, residual_out, False, "add_rms_norm")[0]
+
+
+def add_rms_norm_quantize(x: torch.Tensor, residual: torch.Tensor | None, gamma: torch.Tensor | None, eps: float,
+                          out_dtype: torch.dtype | None = None, *, residual_out: torch.Tensor | None = None):
+    """The same with the normed rows as FP8 rows: (q e4m3, scale fp32 [..., ceil(hidden/128)]), the format of
+    ``quantize_rows``; with ``out_dtype`` also the normed rows themselves, (q, scale, normed) -- a router's gate reads
+    those while the experts read the FP8 rows."""
+    out, q, scale = _norm_call(x, residual, gamma, eps, out_dtype, residual_out, True, "add_rms_norm_quantize")
+    return (q, scale) if out is None else (q, scale, out)
+
+
 def rope_kv_append(qkv, seq_lens, cos, sin, block_table, k_cache, v_cache, *, num_heads, kv_heads, head_dim,
                    block_size, q_out=None):
     """RoPE on Q/K at pos = seq_len - 1 + paged cache append; returns rotated Q (bf16)."""
@@ -347,11 +433,25 @@ def swiglu_act(gate_up: torch.Tensor) -> torch.Tensor:
     return out
 
 
+def swiglu_quantize(gate_up: torch.Tensor):
+    """silu(gate) * up of gate_up bf16/fp32 [rows, 2*inter] (gate columns first) as FP8 rows: (q e4m3 [rows, inter],
+    scale fp32 [rows, ceil(inter/128)])."""
+    dev = _need_cuda(gate_up)
+    if gate_up.dim() != 2 or gate_up.shape[1] < 2 or gate_up.shape[1] % 2 or \
+            gate_up.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError("swiglu_quantize: gate_up must be bf16/fp32 [rows, 2*inter]")
+    rows, inter = gate_up.shape[0], gate_up.shape[1] // 2
+    q = torch.empty(rows, inter, dtype=FP8, device=dev)
+    scale = torch.empty(rows, (inter + 127) // 128, dtype=torch.float32, device=dev)
+    with torch.cuda.device(dev):
+        _lib.check(_lib.load().pto_swiglu_quantize(gate_up.data_ptr(), dtype_code(gate_up.dtype), q.data_ptr(),
+                                                   scale.data_ptr(), rows, inter, _stream_ptr(dev)))
+    return q, scale
+
+
 # ---------------------------------------------------------------------------
 # mixture of experts
 # ---------------------------------------------------------------------------
-
-FP8 = torch.float8_e4m3fn
 
 
 def moe_topk(scores: torch.Tensor, bias: torch.Tensor | None, topk: int, is_logits: bool = False):
@@ -368,6 +468,51 @@ def moe_topk(scores: torch.Tensor, bias: torch.Tensor | None, topk: int, is_logi
         _lib.check(_lib.load().pto_moe_topk(scores.data_ptr(), bias.data_ptr() if bias is not None else None,
                                             1 if is_logits else 0, t, e, topk, idx.data_ptr(), w.data_ptr(),
                                             _stream_ptr(dev)))
+    return idx, w
+
+
+SCORING = {"sigmoid": 0, "softmax": 1}      # PTO_SCORE_*
+
+
+def check_routing(experts: int, topk: int, scoring: str, n_group: int, topk_group: int, group_top: int) -> None:
+    """Raises ValueError for a routing that ``moe_route`` does not compute."""
+    if scoring not in SCORING:
+        raise ValueError(f"scoring must be one of {sorted(SCORING)}, got {scoring!r}")
+    if not 1 <= experts <= 1024:
+        raise ValueError("1..1024 experts")
+    if n_group < 1 or experts % n_group:
+        raise ValueError(f"{experts} experts do not split evenly into {n_group} groups")
+    if not 1 <= topk_group <= n_group:
+        raise ValueError("topk_group must be 1..n_group")
+    if group_top not in (1, 2):
+        raise ValueError("group_top must be 1 or 2")
+    if not 1 <= topk <= min(32, topk_group * (experts // n_group)):
+        raise ValueError("topk must be 1..32 and at most the experts of topk_group groups")
+
+
+def moe_route(logits: torch.Tensor, topk: int, *, bias: torch.Tensor | None = None, scoring: str = "sigmoid",
+              n_group: int = 1, topk_group: int = 1, group_top: int = 2, renormalize: bool = True,
+              route_scale: float = 1.0):
+    """(indices int32 [T, topk], weights fp32 [T, topk]) from gate logits fp32/bf16 [T, experts].
+
+    score = sigmoid or softmax of the logits, key = score + bias; with groups (experts / n_group neighbours each) only
+    the topk_group groups with the largest sum of their best ``group_top`` keys stay; the topk experts by key are listed
+    in descending order, ties to the lower id.  Weight = score, divided by the sum of the chosen scores if
+    ``renormalize``, times ``route_scale``.  A bias of -inf takes an expert out."""
+    dev = _need_cuda(logits) if bias is None else _need_cuda(logits, bias)
+    if logits.dtype not in (torch.float32, torch.bfloat16) or logits.dim() != 2:
+        raise TypeError("moe_route: logits must be fp32 or bf16 [tokens, experts]")
+    t, e = logits.shape
+    check_routing(e, topk, scoring, n_group, topk_group, group_top)
+    if bias is not None and (bias.dtype != torch.float32 or bias.numel() != e):
+        raise ValueError("moe_route: bias must be fp32 [experts]")
+    idx = torch.empty(t, topk, dtype=torch.int32, device=dev)
+    w = torch.empty(t, topk, dtype=torch.float32, device=dev)
+    with torch.cuda.device(dev):
+        _lib.check(_lib.load().pto_moe_route(logits.data_ptr(), dtype_code(logits.dtype),
+                                             bias.data_ptr() if bias is not None else None, SCORING[scoring], t, e, n_group,
+                                             topk_group, group_top, topk, 1 if renormalize else 0, float(route_scale),
+                                             idx.data_ptr(), w.data_ptr(), _stream_ptr(dev)))
     return idx, w
 
 
