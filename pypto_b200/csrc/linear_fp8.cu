@@ -7,6 +7,7 @@
 // It is the dense counterpart of the grouped expert GEMM (the numerics of the reference's block-scaled golden,
 // tests/st/runtime/ops/test_matmul_mx.py:119-131, with fp32 scales per 128).  Products and sums are fp32; out is rounded
 // once.  The order of additions depends on the sizes alone: equal calls give equal bits.
+#include <cstdlib>
 #include "common.cuh"
 #include "kernels.h"
 #include "pair.cuh"
@@ -21,7 +22,7 @@ struct LinFp8Params {
   const float* w_scale;     // [ceil(n / 128), kblocks]
   const float* acc;         // [m, n] or NULL; may be out
   void* out;                // [m, n] bf16 or fp32
-  int m, n, k, kblocks, out_bf16;
+  int m, n, k, kblocks, out_bf16, vec;
   int* err;
 };
 
@@ -29,6 +30,24 @@ __device__ __forceinline__ void store_out(const LinFp8Params& p, size_t o, float
   if (p.acc) v += p.acc[o];
   if (p.out_bf16) static_cast<__nv_bfloat16*>(p.out)[o] = __float2bfloat16_rn(v);
   else static_cast<float*>(p.out)[o] = v;
+}
+
+// Four neighbouring outputs of row m, the first in column n (columns past the end are left alone).
+__device__ __forceinline__ void store_out4(const LinFp8Params& p, int m, int n, float4 v) {
+  const size_t o = static_cast<size_t>(m) * p.n + n;
+  if (p.vec && n + 4 <= p.n) {      // rows of whole 4-element units on whole boundaries
+    if (p.acc) {
+      const float4 a = *reinterpret_cast<const float4*>(p.acc + o);
+      v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
+    }
+    if (p.out_bf16) *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + o) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
+    else *reinterpret_cast<float4*>(static_cast<float*>(p.out) + o) = v;
+  } else {
+    if (n < p.n) store_out(p, o, v.x);
+    if (n + 1 < p.n) store_out(p, o + 1, v.y);
+    if (n + 2 < p.n) store_out(p, o + 2, v.z);
+    if (n + 3 < p.n) store_out(p, o + 3, v.w);
+  }
 }
 
 __device__ __forceinline__ float e4m3_to_f32(uint8_t c) {
@@ -112,10 +131,8 @@ struct Narrow {
   static constexpr uint32_t kTmemCols = kNarrowBufs * BN < 32 ? 32 : kNarrowBufs * BN;
 };
 
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr));
-  return v;
+__device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
 __device__ __forceinline__ float4 lds_f32x4(uint32_t addr) {
   float4 v;
@@ -131,6 +148,8 @@ linear_fp8_narrow_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   float* table = reinterpret_cast<float*>(smem + static_cast<size_t>(stages) * C::kStageBytes);   // [kb_max][kTabStride]
+  float* recv = reinterpret_cast<float*>(smem);            // after the K loop, over the stages: [split][per][128]
+  const int per = (BN + split - 1) / split;                // tokens of the tile that this CTA adds up and stores
   uint64_t* full = reinterpret_cast<uint64_t*>(table + kb_max * C::kTabStride);
   uint64_t* empty = full + kNarrowMaxStages;
   uint64_t* pfull = empty + kNarrowMaxStages;
@@ -264,37 +283,41 @@ linear_fp8_narrow_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_
         acc[j + 3] = fmaf(__uint_as_float(raw[j / 16][j % 16 + 3]), sc.w, acc[j + 3]);
       }
     }
-    const int feat = q * 32 + lane, n = nt * 128 + feat;
-    if (split == 1) {
-      if (n < p.n)
-#pragma unroll
-        for (int j = 0; j < C::kCols; ++j) {
-          const int t = tt * BN + c0 + j;
-          if (t < p.m) store_out(p, static_cast<size_t>(t) * p.n + n, acc[j]);
-        }
-    } else {
-      // every MMA of this CTA has been waited for, so the operand stages are free: [token][feature] partial sums
-      float* part = reinterpret_cast<float*>(smem);
-#pragma unroll
-      for (int j = 0; j < C::kCols; ++j) part[(c0 + j) * 128 + feat] = acc[j];
-    }
   }
   tc_fence_before_sync();
   __syncthreads();
   if (warp == 1) tmem_dealloc(tmem_base, C::kTmemCols);
-  if (split > 1) {
-    cluster_sync_all();
-    const int t1 = min(BN, p.m - tt * BN);
-    if (warp >= 2) {
-      const int feat = (threadIdx.x - 64) & 127, n = nt * 128 + feat;
-      const uint32_t part = smem_u32(smem) + feat * 4;
-      for (int j = rank * (C::kPromoWarps / 4) + ((warp - 2) >> 2); j < t1; j += split * (C::kPromoWarps / 4)) {
-        float v = 0.f;
-        for (int r = 0; r < split; ++r) v += ld_cluster_f32(mapa_u32(part + j * 512, r));   // rank order
-        if (n < p.n) store_out(p, static_cast<size_t>(tt * BN + j) * p.n + n, v);
+  // Token j of the tile is added up by rank j / per: every CTA stores its partial sums there, [rank][token][feature],
+  // over operand stages that no CTA of the cluster reads any more.
+  if (split > 1) cluster_sync_all();
+  if (warp >= 2) {
+    const uint32_t mine = smem_u32(recv) + (rank * per * 128 + q * 32 + lane) * 4;
+    int owner = c0 / per, slot = c0 - owner * per;
+    uint32_t to = split > 1 ? mapa_u32(mine, owner) : mine;
+#pragma unroll
+    for (int j = 0; j < C::kCols; ++j) {
+      st_cluster_f32(to + slot * 512, acc[j]);
+      if (++slot == per && j + 1 < C::kCols) {
+        slot = 0;
+        ++owner;
+        to = mapa_u32(mine, owner);
       }
     }
-    cluster_sync_all();   // no CTA leaves while another may still read its partial sums
+  }
+  if (split > 1) cluster_sync_all();
+  else __syncthreads();
+  if (warp >= 2) {
+    // a warp adds up a token's 128 features, four to a lane, in rank order
+    const int first = tt * BN + rank * per, count = min(min(per, BN - rank * per), p.m - first);
+    for (int t = pw; t < count; t += C::kPromoWarps) {
+      const uint32_t from = smem_u32(recv) + (t * 128 + lane * 4) * 4;
+      float4 v = lds_f32x4(from);
+      for (int r = 1; r < split; ++r) {
+        const float4 a = lds_f32x4(from + r * per * 512);
+        v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
+      }
+      store_out4(p, first + t, nt * 128 + lane * 4, v);
+    }
   }
 }
 
@@ -308,7 +331,7 @@ int narrow_launch(const LinFp8Params& p, int split, cudaStream_t stream) {
   const size_t budget = (C::kCtasPerSm == 2 ? 113 : 227) * 1024;
   int stages = fixed < budget ? static_cast<int>((budget - fixed) / C::kStageBytes) : 0;
   if (stages > kNarrowMaxStages) stages = kNarrowMaxStages;
-  PTO_REQUIRE(stages >= 2 && (split == 1 || static_cast<size_t>(stages) * C::kStageBytes >= BN * 512),
+  PTO_REQUIRE(stages >= 2 && static_cast<size_t>(stages) * C::kStageBytes >= static_cast<size_t>(split) * ((BN + split - 1) / split) * 512,
               "linear_fp8: k does not fit the scale table of a tile");
   // never less than a third of an SM: with at most 256 TMEM columns a CTA, those on one SM cannot ask for more than 512
   const size_t smem = fixed + static_cast<size_t>(stages) * C::kStageBytes;
@@ -342,8 +365,10 @@ int narrow_launch(const LinFp8Params& p, int split, cudaStream_t stream) {
 // K split over up to eight CTAs of a cluster: enough CTAs for the SMs, but whole K blocks (four at least) for each.
 int narrow_split(const LinFp8Params& p, int bn, int ctas_per_sm) {
   const long long tiles = static_cast<long long>((p.m + bn - 1) / bn) * ((p.n + 127) / 128);
-  long long s = (static_cast<long long>(sm_count()) * ctas_per_sm + tiles - 1) / tiles;
-  if (s > p.kblocks / 4) s = p.kblocks / 4;
+  long long s = static_cast<long long>(sm_count()) * ctas_per_sm / tiles;
+  if (const char* e = getenv("LS")) s = atoi(e);
+  static const int mk = [] { const char* e = getenv("MK"); return e ? atoi(e) : 2; }();
+  if (s > p.kblocks / mk) s = p.kblocks / mk;
   return static_cast<int>(s < 1 ? 1 : (s > 8 ? 8 : s));
 }
 
@@ -360,6 +385,7 @@ int linear_fp8_launch(const void* x, const float* x_scale, const void* w, const 
   p.x = static_cast<const uint8_t*>(x); p.x_scale = x_scale; p.w = static_cast<const uint8_t*>(w); p.w_scale = w_scale;
   p.acc = acc; p.out = out; p.m = m; p.n = n; p.k = k; p.kblocks = (k + 127) / 128; p.out_bf16 = out_dtype == PTO_BF16;
   p.err = err;
+  p.vec = n % 4 == 0 && ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(acc)) & 15) == 0;
   const bool tma = k % 16 == 0 && ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w)) & 15) == 0;
   if (tma) {
     if (m <= 16) return narrow_launch<16>(p, narrow_split(p, 16, 2), stream);
