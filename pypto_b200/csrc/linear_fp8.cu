@@ -372,6 +372,306 @@ int narrow_split(const LinFp8Params& p, int bn, int ctas_per_sm) {
   return static_cast<int>(s < 1 ? 1 : (s > 8 ? 8 : s));
 }
 
+// ---------------------------------------------------------------------------
+// Wide tiles on pairs of SMs (tcgen05.mma.cta_group::2): 256 tokens x 256 features.
+//
+// Each CTA of a pair keeps 128 token rows on its TMEM lanes and loads its own rows and half of the weight rows: 32 KB per
+// K block for 128 x 256 x 128 products of its own.  A K block must leave the tensor core on its own, because its scale
+// differs from the next one's: its raw product goes to TMEM and from there, times x_scale[row, kb] * w_scale[128
+// features, kb] -- one number for a thread, which owns one row -- into fp32 registers.  The 256 columns are two
+// halves of 128 with two TMEM buffers each: four promotion warps work for either half, and while one buffer of a half
+// is drained the tensor core fills the other three.  A half has an issuer warp of its own, since one thread takes most
+// of a K block's tensor time to issue its MMAs and commits.
+//   full[s]        in the leader (the even CTA), bytes of both CTAs' loads
+//   empty[s]       in each CTA, two arrivals: the commits of both issuers
+//   pfull[h][b]    in each CTA, the commit of issuer h
+//   pempty[h][b]   in the leader, eight arrivals: four promotion warps of either CTA
+// No load is multicast; every mbarrier wait is bounded; the cluster barriers are reached by every thread on every path.
+// ---------------------------------------------------------------------------
+constexpr int kPairThreads = 12 * 32;                       // producer, two issuers, one idle; eight promotion warps
+// 128 accumulators a thread need more than the 168 registers that 384 threads start with: the first four warps give
+// some of theirs up.  What is asked for afterwards must not be more than the block was launched with, or the
+// request waits for ever: pair_launch checks the kernel's register count.
+constexpr int kPairRegs = 168, kPairRoleRegs = 56, kPairPromoRegs = 224;
+static_assert(128 * kPairRoleRegs + 256 * kPairPromoRegs <= kPairThreads * kPairRegs, "register split");
+constexpr int kPairStages = 6;
+constexpr uint32_t kPairStageBytes = 2 * 128 * 128;
+constexpr uint32_t kPairStoreBytes = 4096;                  // per promotion warp: 32 rows of 128 bytes on their way out
+
+// Waits for the TMEM loads; the registers pass through, so that their uses stay behind the wait.
+__device__ __forceinline__ void tmem_ld_wait_regs(uint32_t (&a)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(a[0]), "+r"(a[1]), "+r"(a[2]), "+r"(a[3]), "+r"(a[4]), "+r"(a[5]), "+r"(a[6]), "+r"(a[7]),
+                 "+r"(a[8]), "+r"(a[9]), "+r"(a[10]), "+r"(a[11]), "+r"(a[12]), "+r"(a[13]), "+r"(a[14]), "+r"(a[15])
+               :
+               : "memory");
+}
+
+__device__ __forceinline__ void sts_u32x4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w, const LinFp8Params p,
+                       int m_tiles, int n_tiles, int group, int vec8, int scale4) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* store = smem + static_cast<size_t>(kPairStages) * kPairStageBytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(store + 8 * kPairStoreBytes);
+  uint64_t* empty = full + kPairStages;
+  uint64_t* pfull = empty + kPairStages;      // [half][buffer]
+  uint64_t* pempty = pfull + 4;
+  uint64_t* drain = pempty + 4;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();          // 0 = leader
+  const int pair = static_cast<int>(blockIdx.x >> 1), npairs = static_cast<int>(gridDim.x >> 1);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kPairStages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 2);
+    }
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&pfull[i], 1);
+      mbar_init(&pempty[i], 8);
+    }
+    mbar_init(&drain[0], 1);
+    mbar_init(&drain[1], 1);
+    fence_barrier_init();
+    tma_prefetch_desc(&tm_x);
+    tma_prefetch_desc(&tm_w);
+  }
+  if (warp == 1) tmem_alloc_pair(tmem_slot, 512);   // the same warp in each CTA of the pair, together
+  tc_fence_before_sync();
+  __syncthreads();
+  cluster_sync_all();              // both CTAs' barriers are initialised before anything is signalled across the pair
+  tc_fence_after_sync();
+  pdl_launch_dependents();         // not before this CTA holds its tensor memory
+  pdl_wait();
+  const uint32_t tmem_base = *tmem_slot;
+  const int tiles = m_tiles * n_tiles;
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPairRoleRegs));
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPairPromoRegs));
+  }
+  if (warp == 0) {
+    // ------------------------------ TMA producer (both CTAs) ------------------------------
+    uint32_t s = 0, ph = 1;
+    bool ok = true;
+    for (int tile = pair; tile < tiles && ok; tile += npairs) {
+      int mt, nt;
+      grouped_tile_coords(tile, group, m_tiles, n_tiles, mt, nt);
+      const int row = mt * 256 + static_cast<int>(rank) * 128, feat = nt * 256 + static_cast<int>(rank) * 64;
+      for (int kb = 0; kb < p.kblocks; ++kb) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&empty[s], ph))) {
+          if (lane == 0) report_error(p.err, kErrBarrierTimeout, 110, kb);
+          ok = false;
+          break;
+        }
+        if (elect_one()) {
+          uint8_t* st = smem + static_cast<size_t>(s) * kPairStageBytes;
+          const uint32_t leader_full = mapa_u32(smem_u32(&full[s]), 0);
+          if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * kPairStageBytes);
+          tma_load_2d_pair(st, &tm_x, kb * 128, row, leader_full);                    // past the matrix: zeros
+          tma_load_2d_pair(st + 16384, &tm_w, kb * 128, feat, leader_full);           // first half: 64 rows of each CTA
+          tma_load_2d_pair(st + 24576, &tm_w, kb * 128, feat + 128, leader_full);     // second half
+        }
+        __syncwarp();
+        if (++s == kPairStages) {
+          s = 0;
+          ph ^= 1u;
+        }
+      }
+    }
+  } else if (warp < 3) {
+    // ------------------------------- MMA issuers (leader only) -------------------------------
+    if (rank == 0) {
+      const uint32_t h = static_cast<uint32_t>(warp - 1);
+      const uint32_t idesc = umma_idesc(256, 128, 0, 0);
+      const uint32_t desc_hi = (1024u >> 4) | (1u << 14) | (2u << 29);   // stride byte offset, version, 128-byte swizzle
+      const uint32_t lo0 = ((smem_u32(smem) & 0x3FFFFu) >> 4) | (1u << 16);
+      const long long my_tiles = pair < tiles ? (tiles - 1 - pair) / npairs + 1 : 0;
+      const uint32_t total = static_cast<uint32_t>(my_tiles * p.kblocks);
+      uint32_t s = 0, ph = 0;
+      for (uint32_t i = 0; i < total; ++i) {
+        const uint32_t b = i & 1u;
+        const bool ok = mbar_wait(&pempty[h * 2 + b], ((i >> 1) & 1u) ^ 1u) && mbar_wait(&full[s], ph);
+        if (!__all_sync(0xffffffffu, ok)) {
+          if (lane == 0) report_error(p.err, kErrBarrierTimeout, 111, static_cast<int>(i));
+          break;
+        }
+        tc_fence_after_sync();
+        if (elect_one()) {
+          const uint32_t x_lo = lo0 + s * (kPairStageBytes >> 4), w_lo = x_lo + ((16384 + h * 8192) >> 4);
+          const uint32_t d = tmem_base + (h * 2 + b) * 128;
+#pragma unroll
+          for (uint32_t k = 0; k < 4; ++k)   // 32 bytes of K per MMA
+            umma_fp8_pair(d, (static_cast<uint64_t>(desc_hi) << 32) | (x_lo + 2 * k),
+                          (static_cast<uint64_t>(desc_hi) << 32) | (w_lo + 2 * k), idesc, k > 0 ? 1u : 0u);
+          umma_commit_pair(&pfull[h * 2 + b]);
+          umma_commit_pair(&empty[s]);
+        }
+        __syncwarp();
+        if (++s == kPairStages) {
+          s = 0;
+          ph ^= 1u;
+        }
+      }
+      // no CTA of the pair releases tensor memory before every MMA has completed, also when a wait gave up
+      if (elect_one()) {
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(&drain[h])) : "memory");
+        if (!mbar_wait(&drain[h], 0)) report_error(p.err, kErrBarrierTimeout, 113, 0);
+      }
+      __syncwarp();
+    }
+  } else if (warp >= 4) {
+    // ------------------------- promotion and epilogue (both CTAs) -------------------------
+    const int pw = warp - 4, h = pw >> 2, q = warp & 3;
+    const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(h) * 256;
+    const uint32_t my_store = smem_u32(store) + pw * kPairStoreBytes;
+    const uint32_t free0 = mapa_u32(smem_u32(&pempty[h * 2]), 0), free1 = mapa_u32(smem_u32(&pempty[h * 2 + 1]), 0);
+    const int n_blocks = (p.n + 127) / 128;
+    uint32_t i = 0;
+    bool ok = true;
+    for (int tile = pair; tile < tiles && ok; tile += npairs) {
+      int mt, nt;
+      grouped_tile_coords(tile, group, m_tiles, n_tiles, mt, nt);
+      const int row0 = mt * 256 + static_cast<int>(rank) * 128 + q * 32, col0 = nt * 256 + h * 128;
+      const float* xs = p.x_scale + static_cast<size_t>(min(row0 + lane, p.m - 1)) * p.kblocks;
+      const float* ws = p.w_scale + static_cast<size_t>(min(nt * 2 + h, n_blocks - 1)) * p.kblocks;
+      unsigned long long acc[64];       // 128 fp32 as packed pairs
+#pragma unroll
+      for (int j = 0; j < 64; ++j) acc[j] = 0ull;
+      float4 x4 = make_float4(0.f, 0.f, 0.f, 0.f), x4n = x4;
+      float xn = 0.f, wn = __ldg(ws);
+      if (scale4) x4n = __ldg(reinterpret_cast<const float4*>(xs));
+      else xn = __ldg(xs);
+      for (int kb = 0; kb < p.kblocks; ++kb, ++i) {
+        // this K block's scale; the next one's (or the next four row scales) are fetched now
+        float x;
+        const int c = kb & 3;
+        if (scale4) {
+          if (c == 0) {
+            x4 = x4n;
+            if (kb + 4 < p.kblocks) x4n = __ldg(reinterpret_cast<const float4*>(xs + kb + 4));
+          }
+          x = c == 0 ? x4.x : (c == 1 ? x4.y : (c == 2 ? x4.z : x4.w));
+        } else {
+          x = xn;
+          if (kb + 1 < p.kblocks) xn = __ldg(xs + kb + 1);
+        }
+        const float sc = x * wn;
+        if (kb + 1 < p.kblocks) wn = __ldg(ws + kb + 1);
+        const unsigned long long s2 = pack_f32x2(sc, sc);
+        const uint32_t b = i & 1u;
+        if (!mbar_wait_warp(&pfull[h * 2 + b], (i >> 1) & 1u)) {
+          if (lane == 0) report_error(p.err, kErrBarrierTimeout, 112, static_cast<int>(i));
+          ok = false;
+          break;
+        }
+        tc_fence_after_sync();
+        const uint32_t t = lane_base + b * 128;
+        uint32_t raw[2][16];
+        tmem_ld_32x16(t, raw[0]);
+#pragma unroll
+        for (int g = 0; g < 8; ++g) {      // sixteen columns at a time, the next sixteen in flight during the products
+          tmem_ld_wait_regs(raw[g & 1]);
+          if (g < 7) {
+            tmem_ld_32x16(t + (g + 1) * 16, raw[(g + 1) & 1]);
+          } else {
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_peer(b ? free1 : free0);
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            fma_f32x2(acc[g * 8 + j], pack_f32x2(__uint_as_float(raw[g & 1][2 * j]), __uint_as_float(raw[g & 1][2 * j + 1])), s2);
+        }
+      }
+      if (!ok) break;
+      // Out through shared memory, 32 rows of 128 bytes at a time (16-byte units swizzled by row), so that a store
+      // instruction writes whole lines: with every lane on a row of its own the stores cost as much as the K loop.
+      if (vec8) {         // bf16, nothing to add: 64 columns at a time
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+#pragma unroll
+          for (int u = 0; u < 8; ++u) {
+            uint32_t o[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              float lo, hi;
+              unpack_f32x2(acc[part * 32 + u * 4 + j], lo, hi);
+              o[j] = pack_bf16x2(lo, hi);
+            }
+            sts_u32x4(my_store + lane * 128 + ((u ^ (lane & 7)) << 4), o[0], o[1], o[2], o[3]);
+          }
+          __syncwarp();
+#pragma unroll
+          for (int r = 0; r < 8; ++r) {
+            const int rr = r * 4 + (lane >> 3), cc = lane & 7, col = col0 + part * 64 + cc * 8;
+            const float4 v = lds_f32x4(my_store + rr * 128 + ((cc ^ (rr & 7)) << 4));
+            if (row0 + rr < p.m && col < p.n)
+              *reinterpret_cast<float4*>(static_cast<__nv_bfloat16*>(p.out) + static_cast<size_t>(row0 + rr) * p.n + col) = v;
+          }
+          __syncwarp();
+        }
+      } else {
+#pragma unroll
+        for (int part = 0; part < 4; ++part) {
+#pragma unroll
+          for (int u = 0; u < 8; ++u) {
+            float v[4];
+            unpack_f32x2(acc[part * 16 + u * 2], v[0], v[1]);
+            unpack_f32x2(acc[part * 16 + u * 2 + 1], v[2], v[3]);
+            sts_u32x4(my_store + lane * 128 + ((u ^ (lane & 7)) << 4), __float_as_uint(v[0]), __float_as_uint(v[1]),
+                      __float_as_uint(v[2]), __float_as_uint(v[3]));
+          }
+          __syncwarp();
+#pragma unroll
+          for (int r = 0; r < 8; ++r) {
+            const int rr = r * 4 + (lane >> 3), cc = lane & 7;
+            const float4 v = lds_f32x4(my_store + rr * 128 + ((cc ^ (rr & 7)) << 4));
+            if (row0 + rr < p.m) store_out4(p, row0 + rr, col0 + part * 32 + cc * 4, v);
+          }
+          __syncwarp();
+        }
+      }
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  cluster_sync_all();   // neither CTA leaves, or frees tensor memory, while its partner may still signal or read it
+  if (warp == 1) tmem_dealloc_pair(tmem_base, 512);
+}
+
+int pair_launch(const LinFp8Params& p, cudaStream_t stream) {
+  const int m_tiles = (p.m + 255) / 256, n_tiles = (p.n + 255) / 256;
+  const long long tiles = static_cast<long long>(m_tiles) * n_tiles;
+  PTO_REQUIRE(tiles * p.kblocks < (1ll << 31), "linear_fp8: problem too large");
+  const int pairs = tiles < sm_count() / 2 ? static_cast<int>(tiles) : sm_count() / 2;
+  const size_t smem = 1024 + static_cast<size_t>(kPairStages) * kPairStageBytes + 8 * kPairStoreBytes + 8 * (2 * kPairStages + 10) + 16;
+  CUtensorMap tm_x, tm_w;
+  int st = make_tensor_map_2d(&tm_x, p.x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.m, p.k, p.k, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (st != kOk) return st;
+  st = make_tensor_map_2d(&tm_w, p.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.n, p.k, p.k, 128, 64, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (st != kOk) return st;
+  static const int regs = [] {
+    cudaFuncAttributes fa;
+    return cudaFuncGetAttributes(&fa, linear_fp8_pair_kernel) == cudaSuccess ? fa.numRegs : 0;
+  }();
+  if (regs < kPairRegs) return fail(kUnsupported, "linear_fp8: the pair kernel has too few registers for its split");
+  if (first_use_on_device(12))
+    PTO_CUDA(cudaFuncSetAttribute(linear_fp8_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
+  const int vec8 = p.out_bf16 && !p.acc && p.n % 8 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
+  const int scale4 = p.kblocks % 4 == 0 && (reinterpret_cast<uintptr_t>(p.x_scale) & 15) == 0;
+  launch_kernel(linear_fp8_pair_kernel, dim3(2 * pairs), dim3(kPairThreads), smem, stream, tm_x, tm_w, p, m_tiles, n_tiles, 16,
+                vec8, scale4);
+  return check_cuda(cudaGetLastError(), "linear_fp8_pair_kernel launch");
+}
+
 }  // namespace
 
 int linear_fp8_launch(const void* x, const float* x_scale, const void* w, const float* w_scale, const float* acc, void* out,
@@ -388,6 +688,8 @@ int linear_fp8_launch(const void* x, const float* x_scale, const void* w, const 
   p.vec = n % 4 == 0 && ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(acc)) & 15) == 0;
   const bool tma = k % 16 == 0 && ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w)) & 15) == 0;
   if (tma) {
+    static const int lp = [] { const char* e = getenv("LP"); return e ? atoi(e) : 1024; }();
+    if (m >= lp) return pair_launch(p, stream);
     if (m <= 16) return narrow_launch<16>(p, narrow_split(p, 16, 2), stream);
     if (m <= 32) return narrow_launch<32>(p, narrow_split(p, 32, 2), stream);
     if (m <= 64) return narrow_launch<64>(p, narrow_split(p, 64, 2), stream);
