@@ -407,13 +407,45 @@ __device__ __forceinline__ void tmem_ld_wait_regs(uint32_t (&a)[16]) {
                : "memory");
 }
 
+// Loads that stay where they are written: the compiler moves an ordinary read-only load down to its use, and a scale that
+// is fetched a K block ahead then arrives a memory latency late (300 of 950 cycles per K block).
+__device__ __forceinline__ float ldg_ahead(const float* p) {
+  float v;
+  asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(v) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ float4 ldg_ahead4(const float* p) {
+  float4 v;
+  asm volatile("ld.global.nc.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p));
+  return v;
+}
+
+template <bool SCALE4>
+__device__ __forceinline__ float4 load_scales(const float* p, int kb, int kblocks) {
+  if (SCALE4) return ldg_ahead4(p + min(kb, kblocks - 4));
+  return make_float4(ldg_ahead(p + min(kb, kblocks - 1)), ldg_ahead(p + min(kb + 1, kblocks - 1)),
+                     ldg_ahead(p + min(kb + 2, kblocks - 1)), ldg_ahead(p + min(kb + 3, kblocks - 1)));
+}
+
 __device__ __forceinline__ void sts_u32x4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
+// Whole-warp wait that polls without suspending and looks at the clock only after many polls (reading the timer costs as
+// much as the usual wait); bounded like mbar_wait.  The vote makes the result warp-uniform.
+__device__ __forceinline__ bool mbar_poll_warp(uint64_t* bar, uint32_t parity) {
+  bool ok = mbar_test_wait(bar, parity);
+#pragma unroll 1
+  for (int i = 0; i < 4096 && !ok; ++i) ok = mbar_test_wait(bar, parity);
+  if (!ok) ok = mbar_spin_wait(bar, parity);
+  return __all_sync(0xffffffffu, ok) != 0;
+}
+
+// SCALE4: K blocks come in fours and the scale arrays are 16-byte aligned, so four scales are one load.
+template <bool SCALE4>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w, const LinFp8Params p,
-                       int m_tiles, int n_tiles, int group, int vec8, int scale4) {
+                       int m_tiles, int n_tiles, int group, int vec8) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* store = smem + static_cast<size_t>(kPairStages) * kPairStageBytes;
@@ -542,35 +574,15 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
       const int row0 = mt * 256 + static_cast<int>(rank) * 128 + q * 32, col0 = nt * 256 + h * 128;
       const float* xs = p.x_scale + static_cast<size_t>(min(row0 + lane, p.m - 1)) * p.kblocks;
       const float* ws = p.w_scale + static_cast<size_t>(min(nt * 2 + h, n_blocks - 1)) * p.kblocks;
-      unsigned long long acc[64];       // 128 fp32 as packed pairs
+      float acc[128];
 #pragma unroll
-      for (int j = 0; j < 64; ++j) acc[j] = 0ull;
-      float4 x4 = make_float4(0.f, 0.f, 0.f, 0.f), x4n = x4;
-      float xn = 0.f, wn = __ldg(ws);
-      if (scale4) x4n = __ldg(reinterpret_cast<const float4*>(xs));
-      else xn = __ldg(xs);
-      for (int kb = 0; kb < p.kblocks; ++kb, ++i) {
-        // this K block's scale; the next one's (or the next four row scales) are fetched now
-        float x;
-        const int c = kb & 3;
-        if (scale4) {
-          if (c == 0) {
-            x4 = x4n;
-            if (kb + 4 < p.kblocks) x4n = __ldg(reinterpret_cast<const float4*>(xs + kb + 4));
-          }
-          x = c == 0 ? x4.x : (c == 1 ? x4.y : (c == 2 ? x4.z : x4.w));
-        } else {
-          x = xn;
-          if (kb + 1 < p.kblocks) xn = __ldg(xs + kb + 1);
-        }
-        const float sc = x * wn;
-        if (kb + 1 < p.kblocks) wn = __ldg(ws + kb + 1);
-        const unsigned long long s2 = pack_f32x2(sc, sc);
-        const uint32_t b = i & 1u;
-        if (!mbar_wait_warp(&pfull[h * 2 + b], (i >> 1) & 1u)) {
+      for (int j = 0; j < 128; ++j) acc[j] = 0.f;
+      // One K block: its raw product times `sc` onto the accumulators; b = its TMEM buffer, ph the phase to wait for.
+      auto block = [&](float sc, uint32_t b, uint32_t ph) {
+        if (!mbar_poll_warp(&pfull[h * 2 + b], ph)) {
           if (lane == 0) report_error(p.err, kErrBarrierTimeout, 112, static_cast<int>(i));
           ok = false;
-          break;
+          return;
         }
         tc_fence_after_sync();
         const uint32_t t = lane_base + b * 128;
@@ -587,8 +599,26 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
             if (lane == 0) mbar_arrive_peer(b ? free1 : free0);
           }
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            fma_f32x2(acc[g * 8 + j], pack_f32x2(__uint_as_float(raw[g & 1][2 * j]), __uint_as_float(raw[g & 1][2 * j + 1])), s2);
+          for (int j = 0; j < 16; ++j) acc[g * 16 + j] = fmaf(__uint_as_float(raw[g & 1][j]), sc, acc[g * 16 + j]);
+        }
+      };
+      // Scales four K blocks at a time, fetched four blocks ahead; what lies past the end is clamped and not used.
+      float4 x4 = load_scales<SCALE4>(xs, 0, p.kblocks), w4 = load_scales<SCALE4>(ws, 0, p.kblocks);
+      for (int kb = 0; kb < p.kblocks && ok; kb += 4) {
+        const float s0 = x4.x * w4.x, s1 = x4.y * w4.y, s2 = x4.z * w4.z, s3 = x4.w * w4.w;
+        x4 = load_scales<SCALE4>(xs, kb + 4, p.kblocks);
+        w4 = load_scales<SCALE4>(ws, kb + 4, p.kblocks);
+        if (SCALE4) {       // a tile starts at a multiple of four K blocks
+          const uint32_t ph = (i >> 1) & 1u;
+          block(s0, 0, ph);
+          if (ok) block(s1, 1, ph);
+          if (ok) block(s2, 0, ph ^ 1u);
+          if (ok) block(s3, 1, ph ^ 1u);
+          i += 4;
+        } else {
+          const int n = min(4, p.kblocks - kb);
+          for (int j = 0; j < n && ok; ++j, ++i)
+            block(j == 0 ? s0 : (j == 1 ? s1 : (j == 2 ? s2 : s3)), i & 1u, (i >> 1) & 1u);
         }
       }
       if (!ok) break;
@@ -601,11 +631,7 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
           for (int u = 0; u < 8; ++u) {
             uint32_t o[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              float lo, hi;
-              unpack_f32x2(acc[part * 32 + u * 4 + j], lo, hi);
-              o[j] = pack_bf16x2(lo, hi);
-            }
+            for (int j = 0; j < 4; ++j) o[j] = pack_bf16x2(acc[part * 64 + u * 8 + 2 * j], acc[part * 64 + u * 8 + 2 * j + 1]);
             sts_u32x4(my_store + lane * 128 + ((u ^ (lane & 7)) << 4), o[0], o[1], o[2], o[3]);
           }
           __syncwarp();
@@ -623,9 +649,7 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
         for (int part = 0; part < 4; ++part) {
 #pragma unroll
           for (int u = 0; u < 8; ++u) {
-            float v[4];
-            unpack_f32x2(acc[part * 16 + u * 2], v[0], v[1]);
-            unpack_f32x2(acc[part * 16 + u * 2 + 1], v[2], v[3]);
+            const float* v = acc + part * 32 + u * 4;
             sts_u32x4(my_store + lane * 128 + ((u ^ (lane & 7)) << 4), __float_as_uint(v[0]), __float_as_uint(v[1]),
                       __float_as_uint(v[2]), __float_as_uint(v[3]));
           }
@@ -659,16 +683,21 @@ int pair_launch(const LinFp8Params& p, cudaStream_t stream) {
   st = make_tensor_map_2d(&tm_w, p.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.n, p.k, p.k, 128, 64, CU_TENSOR_MAP_SWIZZLE_128B);
   if (st != kOk) return st;
   static const int regs = [] {
-    cudaFuncAttributes fa;
-    return cudaFuncGetAttributes(&fa, linear_fp8_pair_kernel) == cudaSuccess ? fa.numRegs : 0;
+    cudaFuncAttributes f4, f1;
+    if (cudaFuncGetAttributes(&f4, linear_fp8_pair_kernel<true>) != cudaSuccess ||
+        cudaFuncGetAttributes(&f1, linear_fp8_pair_kernel<false>) != cudaSuccess)
+      return 0;
+    return f4.numRegs < f1.numRegs ? f4.numRegs : f1.numRegs;
   }();
   if (regs < kPairRegs) return fail(kUnsupported, "linear_fp8: the pair kernel has too few registers for its split");
-  if (first_use_on_device(12))
-    PTO_CUDA(cudaFuncSetAttribute(linear_fp8_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
+  if (first_use_on_device(12)) {
+    PTO_CUDA(cudaFuncSetAttribute(linear_fp8_pair_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
+    PTO_CUDA(cudaFuncSetAttribute(linear_fp8_pair_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
+  }
   const int vec8 = p.out_bf16 && !p.acc && p.n % 8 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
-  const int scale4 = p.kblocks % 4 == 0 && (reinterpret_cast<uintptr_t>(p.x_scale) & 15) == 0;
-  launch_kernel(linear_fp8_pair_kernel, dim3(2 * pairs), dim3(kPairThreads), smem, stream, tm_x, tm_w, p, m_tiles, n_tiles, 16,
-                vec8, scale4);
+  const bool scale4 = p.kblocks % 4 == 0 && ((reinterpret_cast<uintptr_t>(p.x_scale) | reinterpret_cast<uintptr_t>(p.w_scale)) & 15) == 0;
+  launch_kernel(scale4 ? linear_fp8_pair_kernel<true> : linear_fp8_pair_kernel<false>, dim3(2 * pairs), dim3(kPairThreads), smem,
+                stream, tm_x, tm_w, p, m_tiles, n_tiles, 16, vec8);
   return check_cuda(cudaGetLastError(), "linear_fp8_pair_kernel launch");
 }
 
