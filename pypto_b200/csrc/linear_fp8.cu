@@ -431,13 +431,24 @@ __device__ __forceinline__ void sts_u32x4(uint32_t addr, uint32_t a, uint32_t b,
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
-// Whole-warp wait that polls without suspending and looks at the clock only after many polls (reading the timer costs as
-// much as the usual wait); bounded like mbar_wait.  The vote makes the result warp-uniform.
-__device__ __forceinline__ bool mbar_poll_warp(uint64_t* bar, uint32_t parity) {
-  bool ok = mbar_test_wait(bar, parity);
+// Whole-warp wait for the K loop: parked by the hardware for the short time that a try takes without a hint, and bounded
+// by the number of tries instead of the clock.  Reading the timer costs about as much as the usual wait, and polling
+// without parking takes issue slots from the products (2088 instead of 2297 TFLOP/s at 8192 x 28672 x 4096).
+__device__ __forceinline__ bool mbar_try_once(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool mbar_park_warp(uint64_t* bar, uint32_t parity) {
+  bool ok = mbar_try_once(bar, parity);
 #pragma unroll 1
-  for (int i = 0; i < 4096 && !ok; ++i) ok = mbar_test_wait(bar, parity);
-  if (!ok) ok = mbar_spin_wait(bar, parity);
+  for (int i = 0; i < (1 << 20) && !ok; ++i) ok = mbar_try_once(bar, parity);
   return __all_sync(0xffffffffu, ok) != 0;
 }
 
@@ -498,7 +509,7 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
       grouped_tile_coords(tile, group, m_tiles, n_tiles, mt, nt);
       const int row = mt * 256 + static_cast<int>(rank) * 128, feat = nt * 256 + static_cast<int>(rank) * 64;
       for (int kb = 0; kb < p.kblocks; ++kb) {
-        if (!__all_sync(0xffffffffu, mbar_wait(&empty[s], ph))) {
+        if (!mbar_park_warp(&empty[s], ph)) {
           if (lane == 0) report_error(p.err, kErrBarrierTimeout, 110, kb);
           ok = false;
           break;
@@ -530,8 +541,7 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
       uint32_t s = 0, ph = 0;
       for (uint32_t i = 0; i < total; ++i) {
         const uint32_t b = i & 1u;
-        const bool ok = mbar_wait(&pempty[h * 2 + b], ((i >> 1) & 1u) ^ 1u) && mbar_wait(&full[s], ph);
-        if (!__all_sync(0xffffffffu, ok)) {
+        if (!mbar_park_warp(&full[s], ph) || !mbar_park_warp(&pempty[h * 2 + b], ((i >> 1) & 1u) ^ 1u)) {
           if (lane == 0) report_error(p.err, kErrBarrierTimeout, 111, static_cast<int>(i));
           break;
         }
@@ -579,7 +589,7 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
       for (int j = 0; j < 128; ++j) acc[j] = 0.f;
       // One K block: its raw product times `sc` onto the accumulators; b = its TMEM buffer, ph the phase to wait for.
       auto block = [&](float sc, uint32_t b, uint32_t ph) {
-        if (!mbar_poll_warp(&pfull[h * 2 + b], ph)) {
+        if (!mbar_park_warp(&pfull[h * 2 + b], ph)) {
           if (lane == 0) report_error(p.err, kErrBarrierTimeout, 112, static_cast<int>(i));
           ok = false;
           return;
