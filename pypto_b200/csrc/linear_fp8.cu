@@ -7,7 +7,6 @@
 // It is the dense counterpart of the grouped expert GEMM (the numerics of the reference's block-scaled golden,
 // tests/st/runtime/ops/test_matmul_mx.py:119-131, with fp32 scales per 128).  Products and sums are fp32; out is rounded
 // once.  The order of additions depends on the sizes alone: equal calls give equal bits.
-#include <cstdlib>
 #include "common.cuh"
 #include "kernels.h"
 #include "pair.cuh"
@@ -321,14 +320,16 @@ linear_fp8_narrow_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_
   }
 }
 
+size_t narrow_fixed_bytes(int bn, int kb_max);
+size_t narrow_budget(int bn);
+
 template <int BN>
 int narrow_launch(const LinFp8Params& p, int split, cudaStream_t stream) {
   using C = Narrow<BN>;
   const int token_tiles = (p.m + BN - 1) / BN, feature_tiles = (p.n + 127) / 128;
   const int kb_max = (p.kblocks + split - 1) / split;
-  const size_t fixed = 1024 + sizeof(float) * static_cast<size_t>(kb_max) * C::kTabStride +
-                       8 * (2 * kNarrowMaxStages + 2 * kNarrowBufs + 1) + 16;
-  const size_t budget = (C::kCtasPerSm == 2 ? 113 : 227) * 1024;
+  static_assert(C::kTabStride == BN + 4 && (C::kCtasPerSm == 2) == (BN <= 64), "narrow_split sizes the same tile");
+  const size_t fixed = narrow_fixed_bytes(BN, kb_max), budget = narrow_budget(BN);
   int stages = fixed < budget ? static_cast<int>((budget - fixed) / C::kStageBytes) : 0;
   if (stages > kNarrowMaxStages) stages = kNarrowMaxStages;
   PTO_REQUIRE(stages >= 2 && static_cast<size_t>(stages) * C::kStageBytes >= static_cast<size_t>(split) * ((BN + split - 1) / split) * 512,
@@ -362,14 +363,23 @@ int narrow_launch(const LinFp8Params& p, int split, cudaStream_t stream) {
   return check_cuda(cudaGetLastError(), "linear_fp8_narrow_kernel launch");
 }
 
-// K split over up to eight CTAs of a cluster: enough CTAs for the SMs, but whole K blocks (four at least) for each.
-int narrow_split(const LinFp8Params& p, int bn, int ctas_per_sm) {
+// Shared memory of a CTA without its stages.
+size_t narrow_fixed_bytes(int bn, int kb_max) {
+  return 1024 + sizeof(float) * static_cast<size_t>(kb_max) * (bn + 4) + 8 * (2 * kNarrowMaxStages + 2 * kNarrowBufs + 1) + 16;
+}
+size_t narrow_budget(int bn) { return (bn <= 64 ? 113 : 227) * 1024; }
+
+// K split over up to eight CTAs of a cluster: as many CTAs as run at once (a second round costs its own start-up:
+// m = 1, n = 28672, k = 4096 takes 21 us unsplit and 25 us split in two), two K blocks at least for each.  More when the
+// scale table of a longer part would leave less than three stages.  0: K is too long for this kernel.
+int narrow_split(const LinFp8Params& p, int bn) {
   const long long tiles = static_cast<long long>((p.m + bn - 1) / bn) * ((p.n + 127) / 128);
-  long long s = static_cast<long long>(sm_count()) * ctas_per_sm / tiles;
-  if (const char* e = getenv("LS")) s = atoi(e);
-  static const int mk = [] { const char* e = getenv("MK"); return e ? atoi(e) : 2; }();
-  if (s > p.kblocks / mk) s = p.kblocks / mk;
-  return static_cast<int>(s < 1 ? 1 : (s > 8 ? 8 : s));
+  long long s = static_cast<long long>(sm_count()) * (bn <= 64 ? 2 : 1) / tiles;
+  if (s > p.kblocks / 2) s = p.kblocks / 2;
+  s = s < 1 ? 1 : (s > 8 ? 8 : s);
+  const size_t stage = kWTileBytes + static_cast<size_t>(bn) * 128;
+  while (s <= 8 && narrow_fixed_bytes(bn, static_cast<int>((p.kblocks + s - 1) / s)) + 3 * stage > narrow_budget(bn)) ++s;
+  return s > 8 ? 0 : static_cast<int>(s);
 }
 
 // ---------------------------------------------------------------------------
@@ -711,6 +721,20 @@ int pair_launch(const LinFp8Params& p, cudaStream_t stream) {
   return check_cuda(cudaGetLastError(), "linear_fp8_pair_kernel launch");
 }
 
+// Which tile for more than 64 tokens: the time of either in nanoseconds, from a start-up, a cost per round of tiles and a
+// cost per K block that fit the measurements (us, narrow / pair): m = 256, n = k = 4096 12.4 / 20.7;  512, 4096, 4096
+// 18.7 / 19.4;  1024, 1024, 4096 12.1 / 16.9;  777, 1000, 2000 9.4 / 11.6;  1024, 4096, 4096 36.3 / 17.7;
+// 256, 28672, 4096 71.3 / 34.4.  Up to 64 tokens the narrow tile wins throughout (64, 28672, 4096: 25.4 / 30.3).
+long long narrow_time(const LinFp8Params& p, int bn, int split) {
+  const long long ctas = static_cast<long long>((p.m + bn - 1) / bn) * ((p.n + 127) / 128) * split;
+  const long long slots = static_cast<long long>(sm_count()) * (bn <= 64 ? 2 : 1), rounds = (ctas + slots - 1) / slots;
+  return 2000 + rounds * (3000 + 450ll * ((p.kblocks + split - 1) / split)) + (split > 1 ? 1000 : 0);
+}
+long long pair_time(const LinFp8Params& p) {
+  const long long tiles = static_cast<long long>((p.m + 255) / 256) * ((p.n + 255) / 256), pairs = sm_count() / 2;
+  return 3000 + (tiles + pairs - 1) / pairs * (1500 + 410ll * p.kblocks);
+}
+
 }  // namespace
 
 int linear_fp8_launch(const void* x, const float* x_scale, const void* w, const float* w_scale, const float* acc, void* out,
@@ -727,12 +751,15 @@ int linear_fp8_launch(const void* x, const float* x_scale, const void* w, const 
   p.vec = n % 4 == 0 && ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(acc)) & 15) == 0;
   const bool tma = k % 16 == 0 && ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w)) & 15) == 0;
   if (tma) {
-    static const int lp = [] { const char* e = getenv("LP"); return e ? atoi(e) : 1024; }();
-    if (m >= lp) return pair_launch(p, stream);
-    if (m <= 16) return narrow_launch<16>(p, narrow_split(p, 16, 2), stream);
-    if (m <= 32) return narrow_launch<32>(p, narrow_split(p, 32, 2), stream);
-    if (m <= 64) return narrow_launch<64>(p, narrow_split(p, 64, 2), stream);
-    return narrow_launch<128>(p, narrow_split(p, 128, 1), stream);
+    const int bn = m <= 16 ? 16 : (m <= 32 ? 32 : (m <= 64 ? 64 : 128));
+    const int split = narrow_split(p, bn);
+    if (split == 0 || (m > 64 && pair_time(p) < narrow_time(p, bn, split))) return pair_launch(p, stream);
+    switch (bn) {
+      case 16: return narrow_launch<16>(p, split, stream);
+      case 32: return narrow_launch<32>(p, split, stream);
+      case 64: return narrow_launch<64>(p, split, stream);
+      default: return narrow_launch<128>(p, split, stream);
+    }
   }
   PTO_REQUIRE((m + kAnyTile - 1) / kAnyTile <= 65535, "linear_fp8: too many rows");
   launch_kernel(linear_fp8_any_kernel, dim3((n + kAnyTile - 1) / kAnyTile, (m + kAnyTile - 1) / kAnyTile), dim3(256), 0,
