@@ -51,7 +51,19 @@ def _need_cuda(*tensors: torch.Tensor) -> torch.device:
 
 
 def _stream_ptr(dev: torch.device) -> int:
-    return torch.cuda.current_stream(dev).cuda_stream
+    """torch's current stream on ``dev`` (a tensor's device).  The raw handle: building the Stream object around it
+    takes 2 us, as long as a small kernel."""
+    return torch._C._cuda_getCurrentRawStream(dev.index if dev.index is not None else torch.cuda.current_device())
+
+
+def _launch(dev: torch.device, entry, *args) -> None:
+    """One call into the library with ``dev`` as the current device (which it nearly always is: the context manager
+    costs 1.4 us)."""
+    if torch._C._cuda_getDevice() == dev.index:
+        _lib.check(entry(*args))
+    else:
+        with torch.cuda.device(dev):
+            _lib.check(entry(*args))
 
 
 def scratch(dev: torch.device, nbytes: int) -> torch.Tensor:
@@ -254,11 +266,9 @@ def linear_fp8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale:
         raise ValueError("linear_fp8: out must be a bf16 or fp32 [m, n] tensor")
     if acc is not None and (acc.dtype != torch.float32 or tuple(acc.shape) != (m, n)):
         raise ValueError("linear_fp8: acc must be fp32 [m, n]")
-    with torch.cuda.device(dev):
-        _lib.check(_lib.load().pto_linear_fp8(
-            x.data_ptr(), x_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(),
+    _launch(dev, _lib.load().pto_linear_fp8, x.data_ptr(), x_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(),
             acc.data_ptr() if acc is not None else None, out.data_ptr(), dtype_code(out.dtype), m, n, k, _err_ptr(dev),
-            _stream_ptr(dev)))
+            _stream_ptr(dev))
     return out
 
 
@@ -333,12 +343,13 @@ def rms_norm(x: torch.Tensor, gamma: torch.Tensor | None, eps: float, out_dtype:
 
 def _norm_call(x, residual, gamma, eps, out_dtype, residual_out, quantize: bool, name: str):
     dev = _need_cuda(*[t for t in (x, residual, gamma, residual_out) if t is not None])
-    if x.dim() < 1 or x.shape[-1] < 1 or x.dtype not in (torch.bfloat16, torch.float32):
+    shape = x.shape
+    if len(shape) < 1 or shape[-1] < 1 or x.dtype not in (torch.bfloat16, torch.float32):
         raise TypeError(f"{name}: x must be bf16 or fp32 [..., hidden]")
-    hidden = x.shape[-1]
+    hidden = shape[-1]
     rows = x.numel() // hidden
     for t, what in ((residual, "residual"), (residual_out, "residual_out")):
-        if t is not None and (t.shape != x.shape or t.dtype not in (torch.bfloat16, torch.float32)):
+        if t is not None and (t.shape != shape or t.dtype not in (torch.bfloat16, torch.float32)):
             raise ValueError(f"{name}: {what} must be bf16 or fp32 with the shape of x")
     if residual is not None and residual_out is not None and residual.dtype != residual_out.dtype:
         raise ValueError(f"{name}: residual and residual_out must have one dtype")
@@ -349,17 +360,16 @@ def _norm_call(x, residual, gamma, eps, out_dtype, residual_out, quantize: bool,
     if residual_out is None:
         residual_out = residual
     stored = residual if residual is not None else residual_out
-    out = torch.empty(x.shape, dtype=out_dtype, device=dev) if out_dtype is not None else None
-    q = torch.empty(x.shape, dtype=FP8, device=dev) if quantize else None
-    scale = torch.empty(*x.shape[:-1], (hidden + 127) // 128, dtype=torch.float32, device=dev) if quantize else None
-    with torch.cuda.device(dev):
-        _lib.check(_lib.load().pto_add_rms_norm(
+    out = torch.empty(shape, dtype=out_dtype, device=dev) if out_dtype is not None else None
+    q = torch.empty(shape, dtype=FP8, device=dev) if quantize else None
+    scale = torch.empty((*shape[:-1], (hidden + 127) // 128), dtype=torch.float32, device=dev) if quantize else None
+    _launch(dev, _lib.load().pto_add_rms_norm,
             x.data_ptr(), dtype_code(x.dtype), residual.data_ptr() if residual is not None else None,
             residual_out.data_ptr() if residual_out is not None else None,
             dtype_code(stored.dtype) if stored is not None else _lib.PTO_FP32,
             gamma.data_ptr() if gamma is not None else None, out.data_ptr() if out is not None else None,
             dtype_code(out_dtype) if out is not None else _lib.PTO_BF16, q.data_ptr() if quantize else None,
-            scale.data_ptr() if quantize else None, rows, hidden, float(eps), _stream_ptr(dev)))
+            scale.data_ptr() if quantize else None, rows, hidden, float(eps), _stream_ptr(dev))
     return out, q, scale
 
 
@@ -443,9 +453,8 @@ def swiglu_quantize(gate_up: torch.Tensor):
     rows, inter = gate_up.shape[0], gate_up.shape[1] // 2
     q = torch.empty(rows, inter, dtype=FP8, device=dev)
     scale = torch.empty(rows, (inter + 127) // 128, dtype=torch.float32, device=dev)
-    with torch.cuda.device(dev):
-        _lib.check(_lib.load().pto_swiglu_quantize(gate_up.data_ptr(), dtype_code(gate_up.dtype), q.data_ptr(),
-                                                   scale.data_ptr(), rows, inter, _stream_ptr(dev)))
+    _launch(dev, _lib.load().pto_swiglu_quantize, gate_up.data_ptr(), dtype_code(gate_up.dtype), q.data_ptr(),
+            scale.data_ptr(), rows, inter, _stream_ptr(dev))
     return q, scale
 
 
@@ -508,11 +517,9 @@ def moe_route(logits: torch.Tensor, topk: int, *, bias: torch.Tensor | None = No
         raise ValueError("moe_route: bias must be fp32 [experts]")
     idx = torch.empty(t, topk, dtype=torch.int32, device=dev)
     w = torch.empty(t, topk, dtype=torch.float32, device=dev)
-    with torch.cuda.device(dev):
-        _lib.check(_lib.load().pto_moe_route(logits.data_ptr(), dtype_code(logits.dtype),
-                                             bias.data_ptr() if bias is not None else None, SCORING[scoring], t, e, n_group,
-                                             topk_group, group_top, topk, 1 if renormalize else 0, float(route_scale),
-                                             idx.data_ptr(), w.data_ptr(), _stream_ptr(dev)))
+    _launch(dev, _lib.load().pto_moe_route, logits.data_ptr(), dtype_code(logits.dtype),
+            bias.data_ptr() if bias is not None else None, SCORING[scoring], t, e, n_group, topk_group, group_top, topk,
+            1 if renormalize else 0, float(route_scale), idx.data_ptr(), w.data_ptr(), _stream_ptr(dev))
     return idx, w
 
 
