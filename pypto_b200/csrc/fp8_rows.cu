@@ -90,7 +90,8 @@ __global__ void __launch_bounds__(kRowThreads) add_rms_norm_any_kernel(const Add
 }
 
 // a = g * sigmoid(g) * u with the sigmoid as recip(1 + exp(-g)) (examples/models/qwen3_jit/kernels/mlp.py:23-61)
-__device__ __forceinline__ float swiglu(float g, float u) { return g / (1.f + __expf(-g)) * u; }
+// The quotient is the approximate one (2 ulp), as in the GEMMs' epilogues.
+__device__ __forceinline__ float swiglu(float g, float u) { return __fdividef(g, 1.f + __expf(-g)) * u; }
 
 // Any size and alignment: one warp per (row, 128 columns).
 template <typename T>
@@ -122,6 +123,151 @@ swiglu_quantize_any_kernel(const T* __restrict__ gate_up, uint8_t* __restrict__ 
   }
 }
 
+// ---------------------------------------------------------------------------
+// Rows of whole 8-element units on 16-byte boundaries: one read and one write of everything.
+//
+// A thread keeps V units of eight neighbouring elements of its row in registers between the two passes (sum of squares;
+// scaling and quantisation), so 16 neighbouring threads hold one group of 128 columns and its maximum is four shuffles.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ void ld8(const float* p, float (&v)[8]) {
+  const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+__device__ __forceinline__ void unpack8(uint4 w, float (&v)[8]) {
+  v[0] = bf16_lo_to_float(w.x); v[1] = bf16_hi_to_float(w.x); v[2] = bf16_lo_to_float(w.y); v[3] = bf16_hi_to_float(w.y);
+  v[4] = bf16_lo_to_float(w.z); v[5] = bf16_hi_to_float(w.z); v[6] = bf16_lo_to_float(w.w); v[7] = bf16_hi_to_float(w.w);
+}
+__device__ __forceinline__ void ld8(const __nv_bfloat16* p, float (&v)[8]) { unpack8(__ldg(reinterpret_cast<const uint4*>(p)), v); }
+__device__ __forceinline__ void st8(float* p, const float (&v)[8]) {
+  reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+  reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+}
+__device__ __forceinline__ void st8(__nv_bfloat16* p, const float (&v)[8]) {
+  *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+}
+// The residual may be written in place: plain loads, not through the read-only path.
+__device__ __forceinline__ void ld8_rw(const float* p, float (&v)[8]) {
+  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+__device__ __forceinline__ void ld8_rw(const __nv_bfloat16* p, float (&v)[8]) { unpack8(*reinterpret_cast<const uint4*>(p), v); }
+
+__device__ __forceinline__ float group_max16(const float (&v)[8]) {
+  float m = fmaxf(fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3]))),
+                  fmaxf(fmaxf(fabsf(v[4]), fabsf(v[5])), fmaxf(fabsf(v[6]), fabsf(v[7]))));
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));   // within 16 lanes
+  return m;
+}
+
+template <typename TX, typename TR, int V, int THREADS>
+__global__ void __launch_bounds__(THREADS) add_rms_norm_kernel(const AddNormParams p) {
+  __shared__ float red[32];
+  pdl_launch_dependents();
+  pdl_wait();
+  const size_t base = static_cast<size_t>(blockIdx.x) * p.hidden;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const TX* x = static_cast<const TX*>(p.x) + base;
+  const TR* r = p.residual ? static_cast<const TR*>(p.residual) + base : nullptr;
+  TR* ro = p.residual_out ? static_cast<TR*>(p.residual_out) + base : nullptr;
+  float h[V][8];
+#pragma unroll
+  for (int u = 0; u < V; ++u) {
+    const int c = (u * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x)) * 8;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) h[u][j] = 0.f;
+    if (c < p.hidden) ld8(x + c, h[u]);
+  }
+  if (r)
+#pragma unroll
+    for (int u = 0; u < V; ++u) {
+      const int c = (u * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x)) * 8;
+      float v[8] = {};
+      if (c < p.hidden) ld8_rw(r + c, v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) h[u][j] += v[j];
+    }
+  float ss = 0.f;
+#pragma unroll
+  for (int u = 0; u < V; ++u) {
+    const int c = (u * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x)) * 8;
+    if (ro && c < p.hidden) st8(ro + c, h[u]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) ss += h[u][j] * h[u][j];
+  }
+  ss = warp_sum(ss);
+  if (lane == 0) red[warp] = ss;
+  __syncthreads();
+  ss = warp_sum(lane < warps ? red[lane] : 0.f);
+  const float inv = rsqrtf(ss / static_cast<float>(p.hidden) + p.eps);
+#pragma unroll
+  for (int u = 0; u < V; ++u) {
+    const int unit = u * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x), c = unit * 8;
+    const bool in = c < p.hidden;
+    float y[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] = h[u][j] * inv;
+    if (p.gamma && in) {
+      float g[8];
+      ld8(p.gamma + c, g);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] *= g[j];
+    }
+    if (p.out && in) {
+      if (p.out_bf16) st8(static_cast<__nv_bfloat16*>(p.out) + base + c, y);
+      else st8(static_cast<float*>(p.out) + base + c, y);
+    }
+    if (p.q) {
+      const float s = e4m3_group_scale(group_max16(y));
+      if (in) {
+        *reinterpret_cast<uint2*>(p.q + base + c) = e4m3x8(y, s);
+        if ((threadIdx.x & 15) == 0) p.scale[static_cast<size_t>(blockIdx.x) * p.groups + unit / 16] = s;
+      }
+    }
+  }
+}
+
+// Sixteen lanes to a group of 128 columns, U pairs of groups in flight per warp.
+template <typename T, int U>
+__global__ void __launch_bounds__(kRowThreads)
+swiglu_quantize_kernel(const T* __restrict__ gate_up, uint8_t* __restrict__ q, float* __restrict__ scale, int total, int inter,
+                       int groups) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int lane = threadIdx.x & 31, half = lane >> 4, hl = lane & 15;
+  const int warp = static_cast<int>(blockIdx.x) * (kRowThreads / 32) + (threadIdx.x >> 5);
+  const int warps = static_cast<int>(gridDim.x) * (kRowThreads / 32);
+  for (long long g0 = static_cast<long long>(warp) * (2 * U); g0 < total; g0 += static_cast<long long>(warps) * (2 * U)) {
+    float a[U][8], b[U][8];
+    size_t o[U];
+    bool in[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int g = static_cast<int>(g0) + 2 * u + half;
+      const int r = g / groups, c = (g - r * groups) * kQuantGroup + hl * 8;
+      in[u] = g < total && c < inter;
+      o[u] = static_cast<size_t>(r) * inter + c;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) a[u][j] = b[u][j] = 0.f;
+      if (in[u]) {
+        const T* src = gate_up + static_cast<size_t>(r) * 2 * inter + c;
+        ld8(src, a[u]);
+        ld8(src + inter, b[u]);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) a[u][j] = swiglu(a[u][j], b[u][j]);
+      const float s = e4m3_group_scale(group_max16(a[u]));
+      if (in[u]) {
+        *reinterpret_cast<uint2*>(q + o[u]) = e4m3x8(a[u], s);
+        if (hl == 0) scale[static_cast<int>(g0) + 2 * u + half] = s;
+      }
+    }
+  }
+}
+
 template <typename TX, typename TR>
 int add_norm_any(const AddNormParams& p, long long rows, cudaStream_t stream) {
   const size_t smem = sizeof(float) * static_cast<size_t>(p.hidden);
@@ -130,6 +276,31 @@ int add_norm_any(const AddNormParams& p, long long rows, cudaStream_t stream) {
                                   kMaxHidden * 4));
   launch_kernel(add_rms_norm_any_kernel<TX, TR>, dim3(static_cast<unsigned>(rows)), dim3(kRowThreads), smem, stream, p);
   return check_cuda(cudaGetLastError(), "add_rms_norm_any_kernel launch");
+}
+
+template <typename TX, typename TR, int V, int THREADS>
+int add_norm_units(const AddNormParams& p, long long rows, int threads, cudaStream_t stream) {
+  launch_kernel(add_rms_norm_kernel<TX, TR, V, THREADS>, dim3(static_cast<unsigned>(rows)), dim3(threads), 0, stream, p);
+  return check_cuda(cudaGetLastError(), "add_rms_norm_kernel launch");
+}
+
+template <typename TX, typename TR>
+int add_norm(const AddNormParams& p, long long rows, cudaStream_t stream) {
+  const uintptr_t all = reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.residual) |
+                        reinterpret_cast<uintptr_t>(p.residual_out) | reinterpret_cast<uintptr_t>(p.gamma) |
+                        reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.q);
+  const int units = p.hidden / 8;
+  if (p.hidden % 8 != 0 || (all & 15) != 0 || units > 2048) return add_norm_any<TX, TR>(p, rows, stream);
+  // Few rows: as many threads as there are units, the row is latency.  Many rows: 256 threads with several units each, so
+  // that more bytes of more rows are under way.
+  auto whole_warps = [](int n) { return (n + 31) / 32 * 32; };
+  if (units <= 256) return add_norm_units<TX, TR, 1, 256>(p, rows, whole_warps(units), stream);
+  if (rows <= 2ll * sm_count())
+    return units <= 1024 ? add_norm_units<TX, TR, 1, 1024>(p, rows, whole_warps(units), stream)
+                         : add_norm_units<TX, TR, 2, 1024>(p, rows, whole_warps((units + 1) / 2), stream);
+  if (units <= 512) return add_norm_units<TX, TR, 2, 256>(p, rows, whole_warps((units + 1) / 2), stream);
+  if (units <= 1024) return add_norm_units<TX, TR, 4, 256>(p, rows, whole_warps((units + 3) / 4), stream);
+  return add_norm_units<TX, TR, 4, 512>(p, rows, whole_warps((units + 3) / 4), stream);
 }
 
 }  // namespace
@@ -152,9 +323,9 @@ int add_rms_norm_launch(const void* x, int x_dtype, const void* residual, void* 
   p.q = static_cast<uint8_t*>(q); p.scale = scale;
   p.hidden = hidden; p.groups = (hidden + kQuantGroup - 1) / kQuantGroup; p.out_bf16 = out_dtype == PTO_BF16; p.eps = eps;
   if (x_dtype == PTO_BF16)
-    return res_dtype == PTO_BF16 ? add_norm_any<__nv_bfloat16, __nv_bfloat16>(p, rows, stream)
-                                 : add_norm_any<__nv_bfloat16, float>(p, rows, stream);
-  return res_dtype == PTO_BF16 ? add_norm_any<float, __nv_bfloat16>(p, rows, stream) : add_norm_any<float, float>(p, rows, stream);
+    return res_dtype == PTO_BF16 ? add_norm<__nv_bfloat16, __nv_bfloat16>(p, rows, stream)
+                                 : add_norm<__nv_bfloat16, float>(p, rows, stream);
+  return res_dtype == PTO_BF16 ? add_norm<float, __nv_bfloat16>(p, rows, stream) : add_norm<float, float>(p, rows, stream);
 }
 
 int swiglu_quantize_launch(const void* gate_up, int dtype, void* q, float* scale, long long rows, int inter,
@@ -164,6 +335,20 @@ int swiglu_quantize_launch(const void* gate_up, int dtype, void* q, float* scale
   if (rows == 0) return kOk;
   PTO_REQUIRE(gate_up && q && scale, "swiglu_quantize: NULL tensor");
   const int groups = (inter + kQuantGroup - 1) / kQuantGroup;
+  const long long total = rows * groups;
+  if (inter % 8 == 0 && ((reinterpret_cast<uintptr_t>(gate_up) | reinterpret_cast<uintptr_t>(q)) & 15) == 0 &&
+      total < (1ll << 31) - (1 << 24)) {
+    constexpr int kU = 2;
+    const long long want = (total + 2 * kU * (kRowThreads / 32) - 1) / (2 * kU * (kRowThreads / 32)), most = static_cast<long long>(sm_count()) * 8;
+    const dim3 g(static_cast<unsigned>(want < most ? want : most));
+    if (dtype == PTO_BF16)
+      launch_kernel(swiglu_quantize_kernel<__nv_bfloat16, kU>, g, dim3(kRowThreads), 0, stream,
+                    static_cast<const __nv_bfloat16*>(gate_up), static_cast<uint8_t*>(q), scale, static_cast<int>(total), inter, groups);
+    else
+      launch_kernel(swiglu_quantize_kernel<float, kU>, g, dim3(kRowThreads), 0, stream, static_cast<const float*>(gate_up),
+                    static_cast<uint8_t*>(q), scale, static_cast<int>(total), inter, groups);
+    return check_cuda(cudaGetLastError(), "swiglu_quantize_kernel launch");
+  }
   const long long ctas = (rows * groups + kRowThreads / 32 - 1) / (kRowThreads / 32), cap = static_cast<long long>(sm_count()) * 8;
   const dim3 grid(static_cast<unsigned>(ctas < cap ? ctas : cap));
   if (dtype == PTO_BF16)
