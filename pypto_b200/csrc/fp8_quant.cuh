@@ -15,25 +15,54 @@ __device__ __forceinline__ float e4m3_group_scale(float amax) {
   const float s = amax / 448.f;
   return s > 0.f ? s : 1.f;
 }
-// Eight neighbouring values -> eight e4m3 codes, the first in the low byte of .x.
+// Scales for which the quotients below come out exactly as a division's; others (also 0-like and infinite ones) divide.
+__device__ __forceinline__ bool e4m3_plain_scale(float s) { return s > 0x1p-70f && s < 0x1p100f; }
+
+// amax / 448 by the same theorem as below, for a maximum well inside the range; the division otherwise.
+__device__ __forceinline__ float e4m3_group_scale_fast(float amax) {
+  constexpr float r = 1.f / 448.f;
+  const float q = amax * r, s = fmaf(-fmaf(q, 448.f, -amax), r, q);
+  return e4m3_plain_scale(q) ? s : e4m3_group_scale(amax);
+}
+
+// Packed pairs of floats (one instruction for two).
+__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// Eight neighbouring values, given NEGATED as four packed pairs -> eight e4m3 codes, the first in the low byte of .x.
 //
-// v / scale rounded as a division rounds it, at three instructions a value instead of a division's dozen: with r the
+// v / scale rounded as a division rounds it, at three operations a value instead of a division's dozen: with r the
 // correctly rounded 1 / scale, q = v r, e = q scale - v (exact in one fma) and q - e r is the correctly rounded quotient
 // (Markstein, "Computation of elementary functions on the IBM RISC System/6000 processor", 1990, theorem 8.3).  That
-// needs e to be exact: a code other than 0 has |v| >= scale 2^-10, so e is a multiple of 2^-56 scale, which the range of
-// scales below keeps above the smallest subnormal.  Other scales (also infinite ones) divide.
-__device__ __forceinline__ uint2 e4m3x8(const float (&v)[8], float scale) {
+// needs e to be exact: a code other than 0 has |v| >= scale 2^-10, so e is a multiple of 2^-56 scale, which
+// e4m3_plain_scale keeps above the smallest subnormal.  Negated values make every sign right, that of a -0 too, without an
+// operation of its own: q = (-v)(-r), e = q scale + (-v), q + e (-r).
+__device__ __forceinline__ uint2 e4m3x8_of_negated(const unsigned long long (&nv)[4], float scale) {
   float q[8];
-  if (scale > 0x1p-70f && scale < 0x1p100f) {
-    const float r = 1.f / scale;
+  if (e4m3_plain_scale(scale)) {
+    const float r = -1.f / scale;
+    const unsigned long long r2 = pack_f32x2(r, r), s2 = pack_f32x2(scale, scale);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float q0 = v[i] * r;
-      q[i] = fmaf(-fmaf(q0, scale, -v[i]), r, q0);     // signs so that a -0 stays one
+    for (int i = 0; i < 4; ++i) {
+      const unsigned long long q0 = mul_f32x2(nv[i], r2);
+      unpack_f32x2(fma2(fma2(q0, s2, nv[i]), r2, q0), q[2 * i], q[2 * i + 1]);
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) q[i] = v[i] / scale;
+    for (int i = 0; i < 4; ++i) {
+      float a, b;
+      unpack_f32x2(nv[i], a, b);
+      q[2 * i] = -a / scale;
+      q[2 * i + 1] = -b / scale;
+    }
   }
   uint32_t c[4];
 #pragma unroll

@@ -129,34 +129,64 @@ swiglu_quantize_any_kernel(const T* __restrict__ gate_up, uint8_t* __restrict__ 
 // A thread keeps V units of eight neighbouring elements of its row in registers between the two passes (sum of squares;
 // scaling and quantisation), so 16 neighbouring threads hold one group of 128 columns and its maximum is four shuffles.
 // ---------------------------------------------------------------------------
-__device__ __forceinline__ void ld8(const float* p, float (&v)[8]) {
-  const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-}
-__device__ __forceinline__ void unpack8(uint4 w, float (&v)[8]) {
-  v[0] = bf16_lo_to_float(w.x); v[1] = bf16_hi_to_float(w.x); v[2] = bf16_lo_to_float(w.y); v[3] = bf16_hi_to_float(w.y);
-  v[4] = bf16_lo_to_float(w.z); v[5] = bf16_hi_to_float(w.z); v[6] = bf16_lo_to_float(w.w); v[7] = bf16_hi_to_float(w.w);
-}
-__device__ __forceinline__ void ld8(const __nv_bfloat16* p, float (&v)[8]) { unpack8(__ldg(reinterpret_cast<const uint4*>(p)), v); }
-__device__ __forceinline__ void st8(float* p, const float (&v)[8]) {
-  reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-  reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-}
-__device__ __forceinline__ void st8(__nv_bfloat16* p, const float (&v)[8]) {
-  *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
-}
-// The residual may be written in place: plain loads, not through the read-only path.
-__device__ __forceinline__ void ld8_rw(const float* p, float (&v)[8]) {
-  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-}
-__device__ __forceinline__ void ld8_rw(const __nv_bfloat16* p, float (&v)[8]) { unpack8(*reinterpret_cast<const uint4*>(p), v); }
+using Pair = unsigned long long;     // two neighbouring fp32 values
 
-__device__ __forceinline__ float group_max16(const float (&v)[8]) {
-  float m = fmaxf(fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3]))),
-                  fmaxf(fmaxf(fabsf(v[4]), fabsf(v[5])), fmaxf(fabsf(v[6]), fabsf(v[7]))));
+__device__ __forceinline__ void pairs_of(uint4 w, Pair (&v)[4]) {      // eight bf16
+  v[0] = pack_f32x2(bf16_lo_to_float(w.x), bf16_hi_to_float(w.x));
+  v[1] = pack_f32x2(bf16_lo_to_float(w.y), bf16_hi_to_float(w.y));
+  v[2] = pack_f32x2(bf16_lo_to_float(w.z), bf16_hi_to_float(w.z));
+  v[3] = pack_f32x2(bf16_lo_to_float(w.w), bf16_hi_to_float(w.w));
+}
+__device__ __forceinline__ void pairs_of(float4 a, float4 b, Pair (&v)[4]) {
+  v[0] = pack_f32x2(a.x, a.y);
+  v[1] = pack_f32x2(a.z, a.w);
+  v[2] = pack_f32x2(b.x, b.y);
+  v[3] = pack_f32x2(b.z, b.w);
+}
+// Eight neighbouring elements as they come from memory, by plain loads: the residual may be written in place.
+template <typename T>
+struct Raw8;
+template <>
+struct Raw8<float> {
+  float4 a, b;
+  __device__ __forceinline__ void load(const float* p) { a = reinterpret_cast<const float4*>(p)[0]; b = reinterpret_cast<const float4*>(p)[1]; }
+  __device__ __forceinline__ void pairs(Pair (&v)[4]) const { pairs_of(a, b, v); }
+};
+template <>
+struct Raw8<__nv_bfloat16> {
+  uint4 a;
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) { a = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void pairs(Pair (&v)[4]) const { pairs_of(a, v); }
+};
+// The same through the read-only path, for what nothing here writes: these loads may run ahead of the stores before them.
+__device__ __forceinline__ void ld8(const float* p, Pair (&v)[4]) {
+  pairs_of(__ldg(reinterpret_cast<const float4*>(p)), __ldg(reinterpret_cast<const float4*>(p) + 1), v);
+}
+__device__ __forceinline__ void ld8(const __nv_bfloat16* p, Pair (&v)[4]) { pairs_of(__ldg(reinterpret_cast<const uint4*>(p)), v); }
+__device__ __forceinline__ void st8(float* p, const Pair (&v)[4]) {
+  reinterpret_cast<ulonglong2*>(p)[0] = make_ulonglong2(v[0], v[1]);
+  reinterpret_cast<ulonglong2*>(p)[1] = make_ulonglong2(v[2], v[3]);
+}
+__device__ __forceinline__ uint32_t bf16_pair(Pair v) {
+  float a, b;
+  unpack_f32x2(v, a, b);
+  return pack_bf16x2(a, b);
+}
+__device__ __forceinline__ void st8(__nv_bfloat16* p, const Pair (&v)[4]) {
+  *reinterpret_cast<uint4*>(p) = make_uint4(bf16_pair(v[0]), bf16_pair(v[1]), bf16_pair(v[2]), bf16_pair(v[3]));
+}
+
+// Largest magnitude of a group of 128 columns held by 16 neighbouring lanes.
+__device__ __forceinline__ float group_max16(const Pair (&v)[4]) {
+  float m = 0.f;
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));   // within 16 lanes
+  for (int i = 0; i < 4; ++i) {
+    float a, b;
+    unpack_f32x2(v[i], a, b);
+    m = fmaxf(m, fmaxf(fabsf(a), fabsf(b)));
+  }
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   return m;
 }
 
@@ -170,100 +200,117 @@ __global__ void __launch_bounds__(THREADS) add_rms_norm_kernel(const AddNormPara
   const TX* x = static_cast<const TX*>(p.x) + base;
   const TR* r = p.residual ? static_cast<const TR*>(p.residual) + base : nullptr;
   TR* ro = p.residual_out ? static_cast<TR*>(p.residual_out) + base : nullptr;
-  float h[V][8];
+  // Everything a thread reads is under way before the first value is used; a unit past the end reads the last one and
+  // counts as zero.
+  Raw8<TX> xr[V];
+  Raw8<TR> rr[V];
 #pragma unroll
   for (int u = 0; u < V; ++u) {
-    const int c = (u * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x)) * 8;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) h[u][j] = 0.f;
-    if (c < p.hidden) ld8(x + c, h[u]);
+    const int c = min((u * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x)) * 8, p.hidden - 8);
+    xr[u].load(x + c);
+    if (r) rr[u].load(r + c);
   }
-  if (r)
+  Pair h[V][4];
 #pragma unroll
-    for (int u = 0; u < V; ++u) {
-      const int c = (u * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x)) * 8;
-      float v[8] = {};
-      if (c < p.hidden) ld8_rw(r + c, v);
+  for (int u = 0; u < V; ++u) {
+    const bool in = (u * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x)) * 8 < p.hidden;
+    xr[u].pairs(h[u]);
+    if (r) {
+      Pair v[4];
+      rr[u].pairs(v);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) h[u][j] += v[j];
+      for (int j = 0; j < 4; ++j) h[u][j] = add2(h[u][j], v[j]);
     }
-  float ss = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) h[u][j] = in ? h[u][j] : 0ull;
+  }
+  Pair s2 = 0ull;
 #pragma unroll
   for (int u = 0; u < V; ++u) {
     const int c = (u * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x)) * 8;
     if (ro && c < p.hidden) st8(ro + c, h[u]);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) ss += h[u][j] * h[u][j];
+    for (int j = 0; j < 4; ++j) s2 = fma2(h[u][j], h[u][j], s2);
   }
-  ss = warp_sum(ss);
+  float ss, odd;
+  unpack_f32x2(s2, ss, odd);
+  ss = warp_sum(ss + odd);
   if (lane == 0) red[warp] = ss;
   __syncthreads();
   ss = warp_sum(lane < warps ? red[lane] : 0.f);
   const float inv = rsqrtf(ss / static_cast<float>(p.hidden) + p.eps);
+  const Pair inv2 = pack_f32x2(inv, inv), minus = pack_f32x2(-1.f, -1.f);
 #pragma unroll
   for (int u = 0; u < V; ++u) {
     const int unit = u * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x), c = unit * 8;
     const bool in = c < p.hidden;
-    float y[8];
+    Pair y[4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = h[u][j] * inv;
+    for (int j = 0; j < 4; ++j) y[j] = mul_f32x2(h[u][j], inv2);
     if (p.gamma && in) {
-      float g[8];
+      Pair g[4];
       ld8(p.gamma + c, g);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] *= g[j];
+      for (int j = 0; j < 4; ++j) y[j] = mul_f32x2(y[j], g[j]);
     }
     if (p.out && in) {
       if (p.out_bf16) st8(static_cast<__nv_bfloat16*>(p.out) + base + c, y);
       else st8(static_cast<float*>(p.out) + base + c, y);
     }
     if (p.q) {
-      const float s = e4m3_group_scale(group_max16(y));
+      const float s = e4m3_group_scale_fast(group_max16(y));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) y[j] = mul_f32x2(y[j], minus);
       if (in) {
-        *reinterpret_cast<uint2*>(p.q + base + c) = e4m3x8(y, s);
+        *reinterpret_cast<uint2*>(p.q + base + c) = e4m3x8_of_negated(y, s);
         if ((threadIdx.x & 15) == 0) p.scale[static_cast<size_t>(blockIdx.x) * p.groups + unit / 16] = s;
       }
     }
   }
 }
 
-// Sixteen lanes to a group of 128 columns, U pairs of groups in flight per warp.
-template <typename T, int U>
+// n / d for 0 <= n < 2^31 as a multiplication: mul = ceil(2^(31 + l) / d) with 2^l >= d overshoots n / d by less than
+// 1 / d.
+struct FastDiv {
+  uint32_t mul, shift, d;
+  explicit FastDiv(uint32_t divisor) : mul(0), shift(0), d(divisor) {
+    uint32_t l = 1;
+    while ((1ull << l) < d) ++l;
+    mul = d > 1 ? static_cast<uint32_t>(((1ull << (31 + l)) + d - 1) / d) : 0;
+    shift = l - 1;
+  }
+  __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return d > 1 ? __umulhi(n, mul) >> shift : n; }
+};
+
+// One pair of groups of 128 columns per warp at a time, sixteen lanes to a group.
+template <typename T>
 __global__ void __launch_bounds__(kRowThreads)
-swiglu_quantize_kernel(const T* __restrict__ gate_up, uint8_t* __restrict__ q, float* __restrict__ scale, int total, int inter,
-                       int groups) {
+swiglu_quantize_kernel(const T* __restrict__ gate_up, uint8_t* __restrict__ q, float* __restrict__ scale, uint32_t total, int inter,
+                       const FastDiv groups) {
   pdl_launch_dependents();
   pdl_wait();
-  const int lane = threadIdx.x & 31, half = lane >> 4, hl = lane & 15;
-  const int warp = static_cast<int>(blockIdx.x) * (kRowThreads / 32) + (threadIdx.x >> 5);
-  const int warps = static_cast<int>(gridDim.x) * (kRowThreads / 32);
-  for (long long g0 = static_cast<long long>(warp) * (2 * U); g0 < total; g0 += static_cast<long long>(warps) * (2 * U)) {
-    float a[U][8], b[U][8];
-    size_t o[U];
-    bool in[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int g = static_cast<int>(g0) + 2 * u + half;
-      const int r = g / groups, c = (g - r * groups) * kQuantGroup + hl * 8;
-      in[u] = g < total && c < inter;
-      o[u] = static_cast<size_t>(r) * inter + c;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) a[u][j] = b[u][j] = 0.f;
-      if (in[u]) {
-        const T* src = gate_up + static_cast<size_t>(r) * 2 * inter + c;
-        ld8(src, a[u]);
-        ld8(src + inter, b[u]);
-      }
+  const int lane = threadIdx.x & 31, hl = lane & 15;
+  const uint32_t step = gridDim.x * (kRowThreads / 32) * 2;
+  for (uint32_t g0 = (blockIdx.x * (kRowThreads / 32) + (threadIdx.x >> 5)) * 2; g0 < total; g0 += step) {
+    const uint32_t g = g0 + (lane >> 4), r = groups(g);
+    const int c = static_cast<int>(g - r * groups.d) * kQuantGroup + hl * 8;
+    const bool in = g < total && c < inter;
+    Pair a[4] = {}, b[4] = {};
+    if (in) {
+      const T* src = gate_up + static_cast<size_t>(r) * 2 * inter + c;
+      ld8(src, a);
+      ld8(src + inter, b);
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) a[u][j] = swiglu(a[u][j], b[u][j]);
-      const float s = e4m3_group_scale(group_max16(a[u]));
-      if (in[u]) {
-        *reinterpret_cast<uint2*>(q + o[u]) = e4m3x8(a[u], s);
-        if (hl == 0) scale[static_cast<int>(g0) + 2 * u + half] = s;
-      }
+    for (int j = 0; j < 4; ++j) {      // negated: g u / (-1 - exp(-g))
+      float g0f, g1f;
+      unpack_f32x2(a[j], g0f, g1f);
+      a[j] = mul_f32x2(pack_f32x2(__fdividef(g0f, -1.f - __expf(-g0f)), __fdividef(g1f, -1.f - __expf(-g1f))), b[j]);
+    }
+    const float s = e4m3_group_scale_fast(group_max16(a));
+    if (in) {
+      *reinterpret_cast<uint2*>(q + static_cast<size_t>(r) * inter + c) = e4m3x8_of_negated(a, s);
+      if (hl == 0) scale[g] = s;
     }
   }
 }
@@ -299,7 +346,7 @@ int add_norm(const AddNormParams& p, long long rows, cudaStream_t stream) {
     return units <= 1024 ? add_norm_units<TX, TR, 1, 1024>(p, rows, whole_warps(units), stream)
                          : add_norm_units<TX, TR, 2, 1024>(p, rows, whole_warps((units + 1) / 2), stream);
   if (units <= 512) return add_norm_units<TX, TR, 2, 256>(p, rows, whole_warps((units + 1) / 2), stream);
-  if (units <= 1024) return add_norm_units<TX, TR, 4, 256>(p, rows, whole_warps((units + 3) / 4), stream);
+  if (units <= 1024) return add_norm_units<TX, TR, 2, 512>(p, rows, whole_warps((units + 1) / 2), stream);
   return add_norm_units<TX, TR, 4, 512>(p, rows, whole_warps((units + 3) / 4), stream);
 }
 
@@ -338,15 +385,14 @@ int swiglu_quantize_launch(const void* gate_up, int dtype, void* q, float* scale
   const long long total = rows * groups;
   if (inter % 8 == 0 && ((reinterpret_cast<uintptr_t>(gate_up) | reinterpret_cast<uintptr_t>(q)) & 15) == 0 &&
       total < (1ll << 31) - (1 << 24)) {
-    constexpr int kU = 2;
-    const long long want = (total + 2 * kU * (kRowThreads / 32) - 1) / (2 * kU * (kRowThreads / 32)), most = static_cast<long long>(sm_count()) * 8;
+    const long long want = (total + 2 * (kRowThreads / 32) - 1) / (2 * (kRowThreads / 32)), most = static_cast<long long>(sm_count()) * 32;
     const dim3 g(static_cast<unsigned>(want < most ? want : most));
     if (dtype == PTO_BF16)
-      launch_kernel(swiglu_quantize_kernel<__nv_bfloat16, kU>, g, dim3(kRowThreads), 0, stream,
-                    static_cast<const __nv_bfloat16*>(gate_up), static_cast<uint8_t*>(q), scale, static_cast<int>(total), inter, groups);
+      launch_kernel(swiglu_quantize_kernel<__nv_bfloat16>, g, dim3(kRowThreads), 0, stream,
+                    static_cast<const __nv_bfloat16*>(gate_up), static_cast<uint8_t*>(q), scale, static_cast<uint32_t>(total), inter, FastDiv(groups));
     else
-      launch_kernel(swiglu_quantize_kernel<float, kU>, g, dim3(kRowThreads), 0, stream, static_cast<const float*>(gate_up),
-                    static_cast<uint8_t*>(q), scale, static_cast<int>(total), inter, groups);
+      launch_kernel(swiglu_quantize_kernel<float>, g, dim3(kRowThreads), 0, stream, static_cast<const float*>(gate_up),
+                    static_cast<uint8_t*>(q), scale, static_cast<uint32_t>(total), inter, FastDiv(groups));
     return check_cuda(cudaGetLastError(), "swiglu_quantize_kernel launch");
   }
   const long long ctas = (rows * groups + kRowThreads / 32 - 1) / (kRowThreads / 32), cap = static_cast<long long>(sm_count()) * 8;
