@@ -341,35 +341,44 @@ def rms_norm(x: torch.Tensor, gamma: torch.Tensor | None, eps: float, out_dtype:
     return out
 
 
+_WIDE = (torch.bfloat16, torch.float32)
+
+
 def _norm_call(x, residual, gamma, eps, out_dtype, residual_out, quantize: bool, name: str):
-    dev = _need_cuda(*[t for t in (x, residual, gamma, residual_out) if t is not None])
+    tensors = [x]
+    for t, what in ((residual, "residual"), (residual_out, "residual_out")):
+        if t is not None:
+            tensors.append(t)
+            if t.dtype not in _WIDE or t.shape != x.shape:
+                raise ValueError(f"{name}: {what} must be bf16 or fp32 with the shape of x")
+    if gamma is not None:
+        tensors.append(gamma)
+    dev = _need_cuda(*tensors)
     shape = x.shape
-    if len(shape) < 1 or shape[-1] < 1 or x.dtype not in (torch.bfloat16, torch.float32):
+    if len(shape) < 1 or shape[-1] < 1 or x.dtype not in _WIDE:
         raise TypeError(f"{name}: x must be bf16 or fp32 [..., hidden]")
     hidden = shape[-1]
-    rows = x.numel() // hidden
-    for t, what in ((residual, "residual"), (residual_out, "residual_out")):
-        if t is not None and (t.shape != shape or t.dtype not in (torch.bfloat16, torch.float32)):
-            raise ValueError(f"{name}: {what} must be bf16 or fp32 with the shape of x")
-    if residual is not None and residual_out is not None and residual.dtype != residual_out.dtype:
-        raise ValueError(f"{name}: residual and residual_out must have one dtype")
     if gamma is not None and (gamma.dtype != torch.float32 or gamma.numel() != hidden):
         raise ValueError(f"{name}: gamma must be fp32 with hidden elements")
-    if out_dtype not in (None, torch.bfloat16, torch.float32):
+    if out_dtype is not None and out_dtype not in _WIDE:
         raise TypeError(f"{name}: the normed rows are bf16 or fp32")
     if residual_out is None:
         residual_out = residual
-    stored = residual if residual is not None else residual_out
-    out = torch.empty(shape, dtype=out_dtype, device=dev) if out_dtype is not None else None
-    q = torch.empty(shape, dtype=FP8, device=dev) if quantize else None
-    scale = torch.empty((*shape[:-1], (hidden + 127) // 128), dtype=torch.float32, device=dev) if quantize else None
+    elif residual is not None and residual.dtype != residual_out.dtype:
+        raise ValueError(f"{name}: residual and residual_out must have one dtype")
+    out = q = scale = None
+    if out_dtype is not None:
+        out = torch.empty(shape, dtype=out_dtype, device=dev)
+    if quantize:
+        q = torch.empty(shape, dtype=FP8, device=dev)
+        scale = torch.empty((*shape[:-1], (hidden + 127) // 128), dtype=torch.float32, device=dev)
     _launch(dev, _lib.load().pto_add_rms_norm,
-            x.data_ptr(), dtype_code(x.dtype), residual.data_ptr() if residual is not None else None,
-            residual_out.data_ptr() if residual_out is not None else None,
-            dtype_code(stored.dtype) if stored is not None else _lib.PTO_FP32,
-            gamma.data_ptr() if gamma is not None else None, out.data_ptr() if out is not None else None,
-            dtype_code(out_dtype) if out is not None else _lib.PTO_BF16, q.data_ptr() if quantize else None,
-            scale.data_ptr() if quantize else None, rows, hidden, float(eps), _stream_ptr(dev))
+            x.data_ptr(), _DT[x.dtype], None if residual is None else residual.data_ptr(),
+            None if residual_out is None else residual_out.data_ptr(),
+            _lib.PTO_FP32 if residual_out is None else _DT[residual_out.dtype],
+            None if gamma is None else gamma.data_ptr(), None if out is None else out.data_ptr(),
+            _lib.PTO_BF16 if out is None else _DT[out_dtype], q.data_ptr() if quantize else None,
+            scale.data_ptr() if quantize else None, x.numel() // hidden, hidden, float(eps), _stream_ptr(dev))
     return out, q, scale
 
 

@@ -59,7 +59,7 @@ def _norm_bound(hidden):
 
 
 NORM_SIZES = [(1, 1), (1, 4096), (3, 7), (5, 130), (2, 1000), (64, 7168), (33, 2048), (7, 128), (4, 1032), (300, 640),
-              (2, 16384), (3, 16392), (2, 20000), (1, 49152)]
+              (2, 16384), (3, 16392), (2, 20000), (1, 49152), (3, 5003), (2, 16383), (5, 2050), (2, 777), (4, 10222)]
 
 
 @pytest.mark.parametrize("rows, hidden", NORM_SIZES)
@@ -175,7 +175,7 @@ def test_add_rms_norm_refusals():
 # swiglu_quantize
 # ---------------------------------------------------------------------------
 
-@pytest.mark.parametrize("rows, inter", [(1, 1), (1, 2048), (3, 100), (5, 136), (64, 2048), (7, 1288), (260, 384), (2, 14336), (9, 5)])
+@pytest.mark.parametrize("rows, inter", [(1, 1), (1, 2048), (3, 100), (5, 136), (64, 2048), (7, 1288), (260, 384), (2, 14336), (9, 5), (3, 5003), (2, 2050), (33, 258)])
 @pytest.mark.parametrize("dt", [BF16, FP32])
 def test_swiglu_quantize(rows, inter, dt):
     ops = _ops()
