@@ -105,6 +105,40 @@ __global__ void __launch_bounds__(256) linear_fp8_any_kernel(const LinFp8Params 
     }
 }
 
+// Whole-warp wait for the K loop: parked by the hardware for the short time that a try takes without a hint, and bounded
+// by the number of tries instead of the clock.  Reading the timer costs about as much as the usual wait, and polling
+// without parking takes issue slots from the products (2088 instead of 2297 TFLOP/s at 8192 x 28672 x 4096).
+__device__ __forceinline__ bool mbar_try_once(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool mbar_park_warp(uint64_t* bar, uint32_t parity) {
+  bool ok = mbar_try_once(bar, parity);
+#pragma unroll 1
+  for (int i = 0; i < (1 << 20) && !ok; ++i) ok = mbar_try_once(bar, parity);
+  return __all_sync(0xffffffffu, ok) != 0;
+}
+
+// Loads that stay where they are written: the compiler moves an ordinary read-only load down to its use, and a scale that
+// is fetched a K block ahead then arrives a memory latency late (300 of 950 cycles per K block).
+__device__ __forceinline__ float ldg_ahead(const float* p) {
+  float v;
+  asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(v) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ float4 ldg_ahead4(const float* p) {
+  float4 v;
+  asm volatile("ld.global.nc.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p));
+  return v;
+}
+
 // ---------------------------------------------------------------------------
 // Narrow tiles: 128 output features on the TMEM lanes, BN tokens in the columns, K split over a cluster.
 //
@@ -250,9 +284,19 @@ linear_fp8_narrow_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_
     // the table: x_scale[token, kb] * w_scale[tile, kb] (tokens past the end read the last row and are not stored)
     constexpr int kPromoThreads = C::kPromoWarps * 32;
     const float* wsp = p.w_scale + static_cast<size_t>(nt) * p.kblocks + kb0;
-    for (int i = threadIdx.x - 64; i < kbs * BN; i += kPromoThreads) {
-      const int j = i / kbs, kb = i - j * kbs, t = min(tt * BN + j, p.m - 1);
-      table[kb * C::kTabStride + j] = __ldg(p.x_scale + static_cast<size_t>(t) * p.kblocks + kb0 + kb) * __ldg(wsp + kb);
+    constexpr int kAhead = 8;      // entries of a thread under way at once: the table is on the way to the first result
+    for (int i0 = threadIdx.x - 64; i0 < kbs * BN; i0 += kAhead * kPromoThreads) {
+      float sx[kAhead], sw[kAhead];
+      int at[kAhead];
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a) {
+        const int i = min(i0 + a * kPromoThreads, kbs * BN - 1), j = i / kbs, kb = i - j * kbs, t = min(tt * BN + j, p.m - 1);
+        at[a] = kb * C::kTabStride + j;
+        sx[a] = ldg_ahead(p.x_scale + static_cast<size_t>(t) * p.kblocks + kb0 + kb);
+        sw[a] = ldg_ahead(wsp + kb);
+      }
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a) table[at[a]] = sx[a] * sw[a];
     }
     named_bar_sync(1, kPromoThreads);
 #pragma unroll
@@ -417,19 +461,6 @@ __device__ __forceinline__ void tmem_ld_wait_regs(uint32_t (&a)[16]) {
                : "memory");
 }
 
-// Loads that stay where they are written: the compiler moves an ordinary read-only load down to its use, and a scale that
-// is fetched a K block ahead then arrives a memory latency late (300 of 950 cycles per K block).
-__device__ __forceinline__ float ldg_ahead(const float* p) {
-  float v;
-  asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(v) : "l"(p));
-  return v;
-}
-__device__ __forceinline__ float4 ldg_ahead4(const float* p) {
-  float4 v;
-  asm volatile("ld.global.nc.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p));
-  return v;
-}
-
 template <bool SCALE4>
 __device__ __forceinline__ float4 load_scales(const float* p, int kb, int kblocks) {
   if (SCALE4) return ldg_ahead4(p + min(kb, kblocks - 4));
@@ -439,27 +470,6 @@ __device__ __forceinline__ float4 load_scales(const float* p, int kb, int kblock
 
 __device__ __forceinline__ void sts_u32x4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
-}
-
-// Whole-warp wait for the K loop: parked by the hardware for the short time that a try takes without a hint, and bounded
-// by the number of tries instead of the clock.  Reading the timer costs about as much as the usual wait, and polling
-// without parking takes issue slots from the products (2088 instead of 2297 TFLOP/s at 8192 x 28672 x 4096).
-__device__ __forceinline__ bool mbar_try_once(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-__device__ __forceinline__ bool mbar_park_warp(uint64_t* bar, uint32_t parity) {
-  bool ok = mbar_try_once(bar, parity);
-#pragma unroll 1
-  for (int i = 0; i < (1 << 20) && !ok; ++i) ok = mbar_try_once(bar, parity);
-  return __all_sync(0xffffffffu, ok) != 0;
 }
 
 // SCALE4: K blocks come in fours and the scale arrays are 16-byte aligned, so four scales are one load.
