@@ -122,7 +122,7 @@ __device__ __forceinline__ bool mbar_try_once(uint64_t* bar, uint32_t parity) {
 __device__ __forceinline__ bool mbar_park_warp(uint64_t* bar, uint32_t parity) {
   bool ok = mbar_try_once(bar, parity);
 #pragma unroll 1
-  for (int i = 0; i < (1 << 20) && !ok; ++i) ok = mbar_try_once(bar, parity);
+  for (int i = 0; i < (1 << 19) && !ok; ++i) ok = mbar_try_once(bar, parity);
   return __all_sync(0xffffffffu, ok) != 0;
 }
 
@@ -750,6 +750,7 @@ long long pair_time(const LinFp8Params& p) {
 int linear_fp8_launch(const void* x, const float* x_scale, const void* w, const float* w_scale, const float* acc, void* out,
                       int out_dtype, int m, int n, int k, int* err, cudaStream_t stream) {
   PTO_REQUIRE(m >= 0 && n > 0 && k > 0, "linear_fp8: n and k must be positive, m not negative");
+  PTO_REQUIRE(m <= (1 << 30) && n <= (1 << 30) && k <= (1 << 30), "linear_fp8: sizes up to 2^30");
   PTO_REQUIRE(out_dtype == PTO_BF16 || out_dtype == PTO_FP32, "linear_fp8: out must be bf16 or fp32");
   if (m == 0) return kOk;
   PTO_REQUIRE(x && x_scale && w && w_scale && out, "linear_fp8: NULL tensor");

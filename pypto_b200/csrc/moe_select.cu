@@ -148,6 +148,10 @@ __global__ void __launch_bounds__(kRouteWarps * 32) moe_route_any_kernel(const R
 // and counts again; more than 32 candidates, too few available experts and infinite or NaN inputs go to route_token_f64.
 // The weights come from the chosen experts' logits with full 32-bit functions, whatever the keys went through.
 //
+// What bounds it is the number of instructions, about 700 warp instructions a token (the 17 MB of logits of the case below
+// are 2.7 us of memory).  Measured, 256 experts, top 8: 16384 tokens 21 us with 4 of 8 groups, 17 us without groups (63 us
+// with everything in 64 bits and a round over all experts per choice); one token 3.3 us.
+//
 // Error of a key: __expf is off by 2 + 1.173 |x| ulp of itself, which a sigmoid turns into at most s (1 - s) (2 + 1.173
 // |x|) 2^-23 < 0.8 * 2^-23; the sum and the approximate quotient add 3 ulp of s <= 1, adding the bias half an ulp of the
 // key: below 5e-7 + 2^-24 |key|.  Softmax: p (2 + 1.173 |x - max|) 2^-23 < 2.5 * 2^-23 for p <= exp(x - max), and the
@@ -294,164 +298,165 @@ __global__ void __launch_bounds__(256, 4) moe_route_kernel(const RouteParams p, 
   };
 
   for (int t = blockIdx.x * warps + warp; t < p.tokens; t += gridDim.x * warps) {
-  const size_t row = static_cast<size_t>(t) * p.experts;
-  // A group border that 32 bits leave open is settled in 64 bits and the token begun again with that answer, so that its
-  // registers are free meanwhile.
-  bool slow = false, settled = false, stays = true;
-  for (bool again = true; again;) {
-    again = false;
-    float x[PER], key[PER];
-    load(t, x);
-    float top = -INFINITY, sum = 0.f;
-    bool odd = false;                              // an input that 32-bit keys do not handle
+    const size_t row = static_cast<size_t>(t) * p.experts;
+    // A group border that 32 bits leave open is settled in 64 bits and the token begun again with that answer, so that its
+    // registers are free meanwhile.
+    bool slow = false, settled = false, stays = true;
+    for (bool again = true; again;) {
+      again = false;
+      float x[PER], key[PER];
+      load(t, x);
+      float top = -INFINITY, sum = 0.f;
+      bool odd = false;                              // an input that 32-bit keys do not handle
 #pragma unroll
-    for (int j = 0; j < PER; ++j) odd |= !(fabsf(x[j]) < INFINITY);
-    if (p.softmax) {
-#pragma unroll
-      for (int j = 0; j < PER; ++j)
-        if (FULL || e0 + j < p.experts) top = fmaxf(top, x[j]);
-      top = warp_max_fast(odd ? 0.f : top);
-#pragma unroll
-      for (int j = 0; j < PER; ++j) {
-        const float v = FULL || e0 + j < p.experts ? expf(x[j] - top) : 0.f;
-        key[j] = v;
-        sum += v;
-      }
-      sum = warp_sum(sum);
-    }
-    const float inv = p.softmax ? 1.f / sum : 0.f;
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      float k = by_logit ? x[j] : (p.softmax ? key[j] * inv : __fdividef(1.f, 1.f + __expf(-x[j])));
-      if (p.bias && (FULL || e0 + j < p.experts)) k += __ldg(p.bias + e0 + j);
-      odd |= !(k < INFINITY);                      // NaN or +inf; -inf takes the expert out
-      key[j] = FULL || e0 + j < p.experts ? k : -INFINITY;
-    }
-    slow = __any_sync(kAll, odd);
-    if (settled) {
-      if (!stays)
-#pragma unroll
-        for (int j = 0; j < PER; ++j) key[j] = -INFINITY;
-    } else if (grouped && !slow) {
-      float b1 = -INFINITY, b2 = -INFINITY;
-#pragma unroll
-      for (int j = 0; j < PER; ++j) {
-        b2 = fmaxf(b2, fminf(b1, key[j]));
-        b1 = fmaxf(b1, key[j]);
-      }
-      for (int o = 1; o < group_lanes; o <<= 1) {
-        const float o1 = __shfl_xor_sync(kAll, b1, o), o2 = __shfl_xor_sync(kAll, b2, o);
-        b2 = fmaxf(fmaxf(b2, o2), fminf(b1, o1));
-        b1 = fmaxf(b1, o1);
-      }
-      const float gs = p.group_top == 2 && b2 > -INFINITY ? b1 + b2 : b1;
-      const int g = lane / group_lanes;
-      int before = 0;
-      for (int o = 0; o < p.n_group; ++o) {
-        const float v = __shfl_sync(kAll, gs, o * group_lanes);
-        before += v > gs || (v == gs && o < g);
-      }
-      const bool in = g < p.n_group;
-      const bool kept = in && before < p.topk_group;
-      // the last group that stays and the first that goes must be further apart than the error of either sum
-      const float lo = -warp_max_fast(kept ? -gs : -INFINITY), hi = warp_max_fast(in && !kept ? gs : -INFINITY);
-      if (lo == -INFINITY) {
-        slow = true;                               // fewer groups with an available expert than stay
-      } else if (hi > -INFINITY && !(lo - hi > 2.f * (kRouteTol + kRouteTolRel * (fabsf(lo) + fabsf(hi))))) {
-        const double total = p.softmax ? route_sum_f64(p, row, lane, top) : 1.0;
-        double d1 = -INFINITY, d2 = -INFINITY;
-#pragma unroll 1
-        for (int e = e0; e < min(e0 + PER, p.experts); ++e) {
-          const double k = route_key_f64(p, row, e, top, total);
-          d2 = fmax(d2, fmin(d1, k));
-          d1 = fmax(d1, k);
-        }
-        stays = route_keeps_f64(p, lane, group_lanes, d1, d2);
-        settled = again = true;
-        continue;
-      }
-      if (!kept)
-#pragma unroll
-        for (int j = 0; j < PER; ++j) key[j] = -INFINITY;
-    }
-    if (!slow) {
-      float m = key[0];
-#pragma unroll
-      for (int j = 1; j < PER; ++j) m = fmaxf(m, key[j]);
-      // the topk-th largest lane maximum, or less where maxima are equal
-      int left = ordered_int(m), at_k = __reduce_max_sync(kAll, left);
-      const float largest = from_ordered(at_k);
-      for (int k = 1; k < p.topk; ++k) {
-        if (left == at_k) left = static_cast<int>(0x80000000u);
-        at_k = __reduce_max_sync(kAll, left);
-      }
-      const float kth = at_k > ordered_int(-FLT_MAX) ? from_ordered(at_k) : -INFINITY;
-      const float tol = kRouteTol + kRouteTolRel * fmaxf(fabsf(largest), kth > -INFINITY ? fabsf(kth) : 0.f);
-      // without topk lanes that hold an available expert every available one is a candidate
-      const float least = kth > -INFINITY ? kth - 2.f * tol : -FLT_MAX;
-      int mine = 0;
-#pragma unroll
-      for (int j = 0; j < PER; ++j) mine += key[j] >= least;
-      int upto = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(kAll, upto, o);
-        if (lane >= o) upto += u;
-      }
-      const int n = __shfl_sync(kAll, upto, 31);
-      slow = n > 32 || n < p.topk;
-      if (!slow) {
-        int at = upto - mine;
+      for (int j = 0; j < PER; ++j) odd |= !(fabsf(x[j]) < INFINITY);
+      if (p.softmax) {
 #pragma unroll
         for (int j = 0; j < PER; ++j)
-          if (key[j] >= least) {
-            cand_key[warp][at] = key[j];
-            cand_x[warp][at] = x[j];
-            cand_id[warp][at] = e0 + j;
-            ++at;
-          }
-        __syncwarp();
-        const float ki = lane < n ? cand_key[warp][lane] : -INFINITY, xi = lane < n ? cand_x[warp][lane] : 0.f;
-        const int id = lane < n ? cand_id[warp][lane] : 0;
-        int rank = 0;                                  // candidates lie in ascending id order: the tie rule is their order
-        for (int j = 0; j < n; ++j) {
-          const float kj = cand_key[warp][j];
-          rank += kj > ki || (kj == ki && j < lane);
+          if (FULL || e0 + j < p.experts) top = fmaxf(top, x[j]);
+        top = warp_max_fast(odd ? 0.f : top);
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+          const float v = FULL || e0 + j < p.experts ? expf(x[j] - top) : 0.f;
+          key[j] = v;
+          sum += v;
         }
-        __syncwarp();
-        if (lane < n) cand_key[warp][rank] = ki;       // in order: a close pair has close neighbours
-        __syncwarp();
-        const bool near = lane + 1 < n && !(cand_key[warp][lane] - cand_key[warp][lane + 1] > 2.f * tol);
-        // logits and scores order alike as long as exp(x - max) is an ordinary number
-        if (by_logit && __any_sync(kAll, lane < n && xi - top < -80.f)) {
-          slow = true;
-        } else if (__any_sync(kAll, near)) {
+        sum = warp_sum(sum);
+      }
+      const float inv = p.softmax ? 1.f / sum : 0.f;
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        float k = by_logit ? x[j] : (p.softmax ? key[j] * inv : __fdividef(1.f, 1.f + __expf(-x[j])));
+        if (p.bias && (FULL || e0 + j < p.experts)) k += __ldg(p.bias + e0 + j);
+        odd |= !(k < INFINITY);                      // NaN or +inf; -inf takes the expert out
+        key[j] = FULL || e0 + j < p.experts ? k : -INFINITY;
+      }
+      slow = __any_sync(kAll, odd);
+      if (settled) {
+        if (!stays)
+#pragma unroll
+          for (int j = 0; j < PER; ++j) key[j] = -INFINITY;
+      } else if (grouped && !slow) {
+        float b1 = -INFINITY, b2 = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+          b2 = fmaxf(b2, fminf(b1, key[j]));
+          b1 = fmaxf(b1, key[j]);
+        }
+        for (int o = 1; o < group_lanes; o <<= 1) {
+          const float o1 = __shfl_xor_sync(kAll, b1, o), o2 = __shfl_xor_sync(kAll, b2, o);
+          b2 = fmaxf(fmaxf(b2, o2), fminf(b1, o1));
+          b1 = fmaxf(b1, o1);
+        }
+        const float gs = p.group_top == 2 && b2 > -INFINITY ? b1 + b2 : b1;
+        const int g = lane / group_lanes;
+        int before = 0;
+        for (int o = 0; o < p.n_group; ++o) {
+          const float v = __shfl_sync(kAll, gs, o * group_lanes);
+          before += v > gs || (v == gs && o < g);
+        }
+        const bool in = g < p.n_group, kept = in && before < p.topk_group;
+        // every group that stays must lie above every one that goes by more than the errors of the two
+        const float err = kRouteTol + kRouteTolRel * (fabsf(b1) + (p.group_top == 2 && b2 > -INFINITY ? fabsf(b2) : 0.f));
+        const float lo = -warp_max_fast(kept ? (gs > -INFINITY ? err - gs : INFINITY) : -INFINITY);
+        const float hi = warp_max_fast(in && !kept && gs > -INFINITY ? gs + err : -INFINITY);
+        if (lo == -INFINITY) {
+          slow = true;                               // fewer groups with an available expert than stay
+        } else if (!(lo > hi)) {
           const double total = p.softmax ? route_sum_f64(p, row, lane, top) : 1.0;
-          const double k64 = lane < n ? route_key_f64(p, row, id, top, total) : 0.0;
-          cand_key64[warp][lane] = k64;
-          __syncwarp();
-          rank = 0;
-          for (int j = 0; j < n; ++j) {
-            const double kj = cand_key64[warp][j];
-            rank += kj > k64 || (kj == k64 && j < lane);
+          double d1 = -INFINITY, d2 = -INFINITY;
+#pragma unroll 1
+          for (int e = e0; e < min(e0 + PER, p.experts); ++e) {
+            const double k = route_key_f64(p, row, e, top, total);
+            d2 = fmax(d2, fmin(d1, k));
+            d1 = fmax(d1, k);
           }
+          stays = route_keeps_f64(p, lane, group_lanes, d1, d2);
+          settled = again = true;
+          continue;
         }
+        if (!kept)
+#pragma unroll
+          for (int j = 0; j < PER; ++j) key[j] = -INFINITY;
+      }
+      if (!slow) {
+        float m = key[0];
+#pragma unroll
+        for (int j = 1; j < PER; ++j) m = fmaxf(m, key[j]);
+        // the topk-th largest lane maximum, or less where maxima are equal
+        int left = ordered_int(m), at_k = __reduce_max_sync(kAll, left);
+        const float largest = from_ordered(at_k);
+        for (int k = 1; k < p.topk; ++k) {
+          if (left == at_k) left = static_cast<int>(0x80000000u);
+          at_k = __reduce_max_sync(kAll, left);
+        }
+        const float kth = at_k > ordered_int(-FLT_MAX) ? from_ordered(at_k) : -INFINITY;
+        const float tol = kRouteTol + kRouteTolRel * fmaxf(fabsf(largest), kth > -INFINITY ? fabsf(kth) : 0.f);
+        // without topk lanes that hold an available expert every available one is a candidate
+        const float least = kth > -INFINITY ? kth - 2.f * tol : -FLT_MAX;
+        int mine = 0;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) mine += key[j] >= least;
+        int upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int u = __shfl_up_sync(kAll, upto, o);
+          if (lane >= o) upto += u;
+        }
+        const int n = __shfl_sync(kAll, upto, 31);
+        slow = n > 32 || n < p.topk;
         if (!slow) {
-          const bool chosen = lane < n && rank < p.topk;
-          float s = 0.f;
-          if (chosen) s = p.softmax ? expf(xi - top) * inv : 1.f / (1.f + expf(-xi));
-          const float picked = warp_sum(s);
-          if (chosen) {
-            const size_t o = static_cast<size_t>(t) * p.topk + rank;
-            p.idx[o] = id;
-            p.weights[o] = (p.renormalize ? (picked > 0.f ? s / picked : 0.f) : s) * p.route_scale;
+          int at = upto - mine;
+#pragma unroll
+          for (int j = 0; j < PER; ++j)
+            if (key[j] >= least) {
+              cand_key[warp][at] = key[j];
+              cand_x[warp][at] = x[j];
+              cand_id[warp][at] = e0 + j;
+              ++at;
+            }
+          __syncwarp();
+          const float ki = lane < n ? cand_key[warp][lane] : -INFINITY, xi = lane < n ? cand_x[warp][lane] : 0.f;
+          const int id = lane < n ? cand_id[warp][lane] : 0;
+          int rank = 0;                                  // candidates lie in ascending id order: the tie rule is their order
+          for (int j = 0; j < n; ++j) {
+            const float kj = cand_key[warp][j];
+            rank += kj > ki || (kj == ki && j < lane);
+          }
+          __syncwarp();
+          if (lane < n) cand_key[warp][rank] = ki;       // in order: a close pair has close neighbours
+          __syncwarp();
+          const bool near = lane + 1 < n && !(cand_key[warp][lane] - cand_key[warp][lane + 1] > 2.f * tol);
+          // logits and scores order alike as long as exp(x - max) is an ordinary number
+          if (by_logit && __any_sync(kAll, lane < n && xi - top < -80.f)) {
+            slow = true;
+          } else if (__any_sync(kAll, near)) {
+            const double total = p.softmax ? route_sum_f64(p, row, lane, top) : 1.0;
+            const double k64 = lane < n ? route_key_f64(p, row, id, top, total) : 0.0;
+            cand_key64[warp][lane] = k64;
+            __syncwarp();
+            rank = 0;
+            for (int j = 0; j < n; ++j) {
+              const double kj = cand_key64[warp][j];
+              rank += kj > k64 || (kj == k64 && j < lane);
+            }
+          }
+          if (!slow) {
+            const bool chosen = lane < n && rank < p.topk;
+            float s = 0.f;
+            if (chosen) s = p.softmax ? expf(xi - top) * inv : 1.f / (1.f + expf(-xi));
+            const float picked = warp_sum(s);
+            if (chosen) {
+              const size_t o = static_cast<size_t>(t) * p.topk + rank;
+              p.idx[o] = id;
+              p.weights[o] = (p.renormalize ? (picked > 0.f ? s / picked : 0.f) : s) * p.route_scale;
+            }
           }
         }
       }
     }
-  }
-  if (slow) route_lanes_f64<PER>(p, t, lane, group_lanes);
-  __syncwarp();                                        // the candidates are read before the next token's are written
+    if (slow) route_lanes_f64<PER>(p, t, lane, group_lanes);
+    __syncwarp();                                      // the candidates are read before the next token's are written
   }
 }
 
@@ -471,7 +476,7 @@ int moe_route_launch(const void* logits, int logits_dtype, const float* bias, in
                      int32_t* idx, float* weights, cudaStream_t stream) {
   PTO_REQUIRE(logits_dtype == PTO_FP32 || logits_dtype == PTO_BF16, "moe_route: logits must be fp32 or bf16");
   PTO_REQUIRE(scoring == PTO_SCORE_SIGMOID || scoring == PTO_SCORE_SOFTMAX, "moe_route: unknown scoring");
-  PTO_REQUIRE(tokens >= 0 && experts > 0 && experts <= kRouteMaxExperts, "moe_route: 1..1024 experts");
+  PTO_REQUIRE(tokens >= 0 && tokens <= (1 << 30) && experts > 0 && experts <= kRouteMaxExperts, "moe_route: 1..1024 experts, at most 2^30 tokens");
   PTO_REQUIRE(n_group > 0 && experts % n_group == 0, "moe_route: the experts must split evenly into n_group groups");
   PTO_REQUIRE(topk_group > 0 && topk_group <= n_group, "moe_route: topk_group must be 1..n_group");
   PTO_REQUIRE(group_top == 1 || group_top == 2, "moe_route: group_top must be 1 or 2");

@@ -39,12 +39,12 @@ def _swiglu(x=P, dt=BF16, q=P, s=P, rows=4, inter=64):
     (_norm, dict(odt=FP16), "out"), (_norm, dict(out=None), "neither"), (_norm, dict(q=P), "both"),
     (_norm, dict(s=P), "both"), (_norm, dict(eps=-1.0), "eps"), (_norm, dict(eps=math.nan), "eps"), (_norm, dict(x=None), "NULL"),
     (_linear, dict(n=0), "positive"), (_linear, dict(k=0), "positive"), (_linear, dict(m=-1), "positive"),
-    (_linear, dict(odt=FP16), "out"), (_linear, dict(x=None), "NULL"), (_linear, dict(ws=None), "NULL"),
+    (_linear, dict(m=(1 << 30) + 1), "2^30"), (_linear, dict(odt=FP16), "out"), (_linear, dict(x=None), "NULL"), (_linear, dict(ws=None), "NULL"),
     (_linear, dict(acc=P), "fp32 out"),
     (_swiglu, dict(dt=FP16), "gate_up"), (_swiglu, dict(inter=0), "sizes"), (_swiglu, dict(rows=-1), "sizes"),
     (_swiglu, dict(q=None), "NULL"),
     (_route, dict(dt=FP16), "logits"), (_route, dict(scoring=2), "scoring"), (_route, dict(experts=1025), "experts"),
-    (_route, dict(experts=0), "experts"), (_route, dict(ng=5, tg=2), "evenly"), (_route, dict(ng=4, tg=5), "topk_group"),
+    (_route, dict(experts=0), "experts"), (_route, dict(tokens=(1 << 30) + 1), "tokens"), (_route, dict(ng=5, tg=2), "evenly"), (_route, dict(ng=4, tg=5), "topk_group"),
     (_route, dict(ng=4, tg=0), "topk_group"), (_route, dict(gt=3), "group_top"), (_route, dict(topk=0), "topk"),
     (_route, dict(topk=33), "topk"), (_route, dict(ng=32, tg=1, topk=3), "topk"), (_route, dict(idx=None), "NULL"),
 ])

@@ -368,6 +368,13 @@ def test_route_masks_and_odd_values(scoring):
     _check_route(logits, 20, bias, scoring=scoring)             # more asked than there are: filled at weight 0
     idx, w = _check_route(logits, 4, torch.full((64,), -inf), scoring=scoring)
     assert idx.cpu().tolist() == [[0, 1, 2, 3]] * 30 and (w == 0).all()
+    low = torch.finfo(FP32).min                                 # the other way to mask: availability by value
+    masked = torch.where(torch.isinf(bias), torch.full_like(bias, low), bias)
+    big = 1e6 * torch.where(torch.rand(64, generator=g) < 0.5, -1.0, 1.0)
+    for b in (masked, big, big + 0.1 * torch.randn(64, generator=g)):
+        for kw in (dict(), dict(n_group=8, topk_group=4, group_top=2), dict(n_group=8, topk_group=3, group_top=1),
+                   dict(n_group=4, topk_group=3, group_top=2)):
+            _check_route(logits, 8, b, scoring=scoring, **kw)
     odd = logits.clone()
     odd[0, 5] = math.nan
     odd[1] = math.nan
