@@ -267,7 +267,7 @@ __device__ __noinline__ void route_lanes_f64(const RouteParams& p, int t, int la
 
 // FULL: every lane holds PER experts.
 template <int PER, bool FULL>
-__global__ void __launch_bounds__(256, 4) moe_route_kernel(const RouteParams p, int group_lanes, int vec) {
+__global__ void __launch_bounds__(256, PER <= 8 ? 4 : 2) moe_route_kernel(const RouteParams p, int group_lanes, int vec) {
   __shared__ float cand_key[8][32], cand_x[8][32];
   __shared__ int cand_id[8][32];
   __shared__ double cand_key64[8][32];
