@@ -148,15 +148,18 @@ __global__ void __launch_bounds__(kRouteWarps * 32) moe_route_any_kernel(const R
 // and counts again; more than 32 candidates, too few available experts and infinite or NaN inputs go to route_token_f64.
 // The weights come from the chosen experts' logits with full 32-bit functions, whatever the keys went through.
 //
-// What bounds it is the number of instructions, about 700 warp instructions a token (the 17 MB of logits of the case below
-// are 2.7 us of memory).  Measured, 256 experts, top 8: 16384 tokens 21 us with 4 of 8 groups, 17 us without groups (63 us
-// with everything in 64 bits and a round over all experts per choice); one token 3.3 us.
+// What bounds it is the number of instructions, 500 to 800 warp instructions a token (the 17 MB of logits of 16384 tokens
+// are 2.7 us of memory).  Measured, 256 experts, top 8: 16384 tokens 20.4 us with 4 of 8 groups, 16.2 us without groups (63 us
+// with everything in 64 bits and a round over all experts per choice), 4096 tokens 7.0 us, one token 3.2 us.  Tried:
+// putting close tokens off to the CTA's end (fewer registers, but 21-22 us: the late ones are a tail), five or six CTAs an
+// SM instead of four (spills, 23-28 us), eight or sixteen rounds of CTAs instead of one resident set (20.5 us, but 7.8-8.4
+// us at 4096 tokens).
 //
 // Error of a key: __expf is off by 2 + 1.173 |x| ulp of itself, which a sigmoid turns into at most s (1 - s) (2 + 1.173
 // |x|) 2^-23 < 0.8 * 2^-23; the sum and the approximate quotient add 3 ulp of s <= 1, adding the bias half an ulp of the
 // key: below 5e-7 + 2^-24 |key|.  Softmax: p (2 + 1.173 |x - max|) 2^-23 < 2.5 * 2^-23 for p <= exp(x - max), and the
-// sum's own error, p * 2^-20: below 1.3e-6 + 2^-24 |key|.  Two keys can be told apart beyond twice that.
-constexpr float kRouteTol = 3e-6f, kRouteTolRel = 2.4e-7f;
+// sum's own error, p * 2^-20: below 1.3e-6 + 2^-24 |key|.  Two keys can be told apart beyond twice that: kTol...
+constexpr float kTolSigmoid = 1.1e-6f, kTolSoftmax = 2.7e-6f, kTolRel = 2.4e-7f;
 
 // Floats as integers of the same order (no NaN), for the integer reductions of a warp.
 __device__ __forceinline__ int ordered_int(float v) {
@@ -268,7 +271,7 @@ __device__ __noinline__ void route_lanes_f64(const RouteParams& p, int t, int la
 // FULL: every lane holds PER experts.
 template <int PER, bool FULL>
 __global__ void __launch_bounds__(256, PER <= 8 ? 4 : 2) moe_route_kernel(const RouteParams p, int group_lanes, int vec) {
-  __shared__ float cand_key[8][32], cand_x[8][32];
+  __shared__ __align__(16) float cand_key[8][32];
   __shared__ int cand_id[8][32];
   __shared__ double cand_key64[8][32];
   pdl_launch_dependents();
@@ -280,22 +283,23 @@ __global__ void __launch_bounds__(256, PER <= 8 ? 4 : 2) moe_route_kernel(const 
   // softmax without bias and groups orders like the logits
   const bool by_logit = p.softmax && !p.bias && !grouped;
 
-  auto load = [&](int t, float (&x)[PER]) {
-    const size_t row = static_cast<size_t>(t) * p.experts;
+  // this lane's experts of a row of fp32 numbers
+  auto load = [&](const float* from, size_t row, bool vectors, float (&x)[PER]) {
     if constexpr (PER % 4 == 0) {
-      if (vec) {
-        const float* src = static_cast<const float*>(p.logits) + row + e0;
+      if (vectors) {
+        const float4* src = reinterpret_cast<const float4*>(from + row + e0);
 #pragma unroll
         for (int j = 0; j < PER; j += 4) {
-          const float4 v = FULL || e0 + j < p.experts ? __ldg(reinterpret_cast<const float4*>(src + j)) : make_float4(0.f, 0.f, 0.f, 0.f);
+          const float4 v = FULL || e0 + j < p.experts ? __ldg(src + j / 4) : make_float4(0.f, 0.f, 0.f, 0.f);
           x[j] = v.x; x[j + 1] = v.y; x[j + 2] = v.z; x[j + 3] = v.w;
         }
         return;
       }
     }
 #pragma unroll
-    for (int j = 0; j < PER; ++j) x[j] = FULL || e0 + j < p.experts ? route_logit(p, row + e0 + j) : 0.f;
+    for (int j = 0; j < PER; ++j) x[j] = FULL || e0 + j < p.experts ? __ldg(from + row + e0 + j) : 0.f;
   };
+  const float tol_abs = p.softmax ? kTolSoftmax : kTolSigmoid;
 
   for (int t = blockIdx.x * warps + warp; t < p.tokens; t += gridDim.x * warps) {
     const size_t row = static_cast<size_t>(t) * p.experts;
@@ -305,7 +309,12 @@ __global__ void __launch_bounds__(256, PER <= 8 ? 4 : 2) moe_route_kernel(const 
     for (bool again = true; again;) {
       again = false;
       float x[PER], key[PER];
-      load(t, x);
+      if (p.logits_bf16) {
+#pragma unroll
+        for (int j = 0; j < PER; ++j) x[j] = FULL || e0 + j < p.experts ? route_logit(p, row + e0 + j) : 0.f;
+      } else {
+        load(static_cast<const float*>(p.logits), row, vec & 1, x);
+      }
       float top = -INFINITY, sum = 0.f;
       bool odd = false;                              // an input that 32-bit keys do not handle
 #pragma unroll
@@ -324,10 +333,17 @@ __global__ void __launch_bounds__(256, PER <= 8 ? 4 : 2) moe_route_kernel(const 
         sum = warp_sum(sum);
       }
       const float inv = p.softmax ? 1.f / sum : 0.f;
+      float bias[PER];
+      if (p.bias) {
+        load(p.bias, 0, vec & 2, bias);
+      } else {
+#pragma unroll
+        for (int j = 0; j < PER; ++j) bias[j] = 0.f;
+      }
 #pragma unroll
       for (int j = 0; j < PER; ++j) {
         float k = by_logit ? x[j] : (p.softmax ? key[j] * inv : __fdividef(1.f, 1.f + __expf(-x[j])));
-        if (p.bias && (FULL || e0 + j < p.experts)) k += __ldg(p.bias + e0 + j);
+        k += bias[j];
         odd |= !(k < INFINITY);                      // NaN or +inf; -inf takes the expert out
         key[j] = FULL || e0 + j < p.experts ? k : -INFINITY;
       }
@@ -348,21 +364,26 @@ __global__ void __launch_bounds__(256, PER <= 8 ? 4 : 2) moe_route_kernel(const 
           b2 = fmaxf(fmaxf(b2, o2), fminf(b1, o1));
           b1 = fmaxf(b1, o1);
         }
-        const float gs = p.group_top == 2 && b2 > -INFINITY ? b1 + b2 : b1;
-        const int g = lane / group_lanes;
-        int before = 0;
-        for (int o = 0; o < p.n_group; ++o) {
-          const float v = __shfl_sync(kAll, gs, o * group_lanes);
-          before += v > gs || (v == gs && o < g);
+        const bool two = p.group_top == 2 && b2 > -INFINITY;
+        const float gs = two ? b1 + b2 : b1;
+        // the topk_group best by as many maxima; equal groups go together, and then there are too many
+        constexpr int kNone = static_cast<int>(0x80000000u);
+        const bool in = lane < p.n_group * group_lanes;
+        const int mine = in ? ordered_int(gs) : kNone;
+        int left = mine, at = kNone;
+        for (int k = 0; k < p.topk_group; ++k) {
+          at = __reduce_max_sync(kAll, left);
+          if (left == at) left = kNone;
         }
-        const bool in = g < p.n_group, kept = in && before < p.topk_group;
-        // every group that stays must lie above every one that goes by more than the errors of the two
-        const float err = kRouteTol + kRouteTolRel * (fabsf(b1) + (p.group_top == 2 && b2 > -INFINITY ? fabsf(b2) : 0.f));
-        const float lo = -warp_max_fast(kept ? (gs > -INFINITY ? err - gs : INFINITY) : -INFINITY);
-        const float hi = warp_max_fast(in && !kept && gs > -INFINITY ? gs + err : -INFINITY);
-        if (lo == -INFINITY) {
+        const bool kept = in && mine >= at;
+        const float lo = from_ordered(at), hi = from_ordered(max(__reduce_max_sync(kAll, left), ordered_int(-FLT_MAX)));
+        // A group that stays must lie above one that goes by more than the errors of both (two keys' each); a sum far
+        // below any choice (a mask's) takes no part.
+        const float err = gs > -1e30f ? tol_abs + kTolRel * (fabsf(b1) + (two ? fabsf(b2) : 0.f)) : 0.f;
+        const float most = __int_as_float(__reduce_max_sync(kAll, in ? __float_as_int(err) : 0));
+        if (at <= ordered_int(-FLT_MAX)) {
           slow = true;                               // fewer groups with an available expert than stay
-        } else if (!(lo > hi)) {
+        } else if (!(lo - hi > 2.f * most) || lo < -1e29f || __popc(__ballot_sync(kAll, kept)) != p.topk_group * group_lanes) {
           const double total = p.softmax ? route_sum_f64(p, row, lane, top) : 1.0;
           double d1 = -INFINITY, d2 = -INFINITY;
 #pragma unroll 1
@@ -391,9 +412,9 @@ __global__ void __launch_bounds__(256, PER <= 8 ? 4 : 2) moe_route_kernel(const 
           at_k = __reduce_max_sync(kAll, left);
         }
         const float kth = at_k > ordered_int(-FLT_MAX) ? from_ordered(at_k) : -INFINITY;
-        const float tol = kRouteTol + kRouteTolRel * fmaxf(fabsf(largest), kth > -INFINITY ? fabsf(kth) : 0.f);
+        const float tol = tol_abs + kTolRel * fmaxf(fabsf(largest), kth > -INFINITY ? fabsf(kth) : 0.f);
         // without topk lanes that hold an available expert every available one is a candidate
-        const float least = kth > -INFINITY ? kth - 2.f * tol : -FLT_MAX;
+        const float least = kth > -INFINITY ? kth - tol : -FLT_MAX;
         int mine = 0;
 #pragma unroll
         for (int j = 0; j < PER; ++j) mine += key[j] >= least;
@@ -411,22 +432,23 @@ __global__ void __launch_bounds__(256, PER <= 8 ? 4 : 2) moe_route_kernel(const 
           for (int j = 0; j < PER; ++j)
             if (key[j] >= least) {
               cand_key[warp][at] = key[j];
-              cand_x[warp][at] = x[j];
               cand_id[warp][at] = e0 + j;
               ++at;
             }
+          if (lane >= n) cand_key[warp][lane] = -INFINITY;
           __syncwarp();
-          const float ki = lane < n ? cand_key[warp][lane] : -INFINITY, xi = lane < n ? cand_x[warp][lane] : 0.f;
+          const float ki = cand_key[warp][lane];
           const int id = lane < n ? cand_id[warp][lane] : 0;
-          int rank = 0;                                  // candidates lie in ascending id order: the tie rule is their order
-          for (int j = 0; j < n; ++j) {
-            const float kj = cand_key[warp][j];
-            rank += kj > ki || (kj == ki && j < lane);
+          const float xi = lane < n ? route_logit(p, row + id) : 0.f;
+          // how many lie above, and how many above or too close to tell (itself among them): equal keys are close
+          const float low = ki - tol;
+          int rank = 0, above = 0;
+          for (int j = 0; j < n; j += 4) {
+            const float4 k4 = *reinterpret_cast<const float4*>(&cand_key[warp][j]);
+            rank += (k4.x > ki) + (k4.y > ki) + (k4.z > ki) + (k4.w > ki);
+            above += (k4.x >= low) + (k4.y >= low) + (k4.z >= low) + (k4.w >= low);
           }
-          __syncwarp();
-          if (lane < n) cand_key[warp][rank] = ki;       // in order: a close pair has close neighbours
-          __syncwarp();
-          const bool near = lane + 1 < n && !(cand_key[warp][lane] - cand_key[warp][lane + 1] > 2.f * tol);
+          const bool near = lane < n && above != rank + 1;
           // logits and scores order alike as long as exp(x - max) is an ordinary number
           if (by_logit && __any_sync(kAll, lane < n && xi - top < -80.f)) {
             slow = true;
@@ -444,7 +466,7 @@ __global__ void __launch_bounds__(256, PER <= 8 ? 4 : 2) moe_route_kernel(const 
           if (!slow) {
             const bool chosen = lane < n && rank < p.topk;
             float s = 0.f;
-            if (chosen) s = p.softmax ? expf(xi - top) * inv : 1.f / (1.f + expf(-xi));
+            if (chosen) s = p.softmax ? expf(xi - top) * inv : __fdividef(1.f, 1.f + expf(-xi));
             const float picked = warp_sum(s);
             if (chosen) {
               const size_t o = static_cast<size_t>(t) * p.topk + rank;
@@ -462,8 +484,10 @@ __global__ void __launch_bounds__(256, PER <= 8 ? 4 : 2) moe_route_kernel(const 
 
 template <int PER>
 int route_launch_per(const RouteParams& p, int group_lanes, cudaStream_t stream) {
-  const int vec = !p.logits_bf16 && p.experts % 4 == 0 && (reinterpret_cast<uintptr_t>(p.logits) & 15) == 0;
-  const int blocks = (p.tokens + 7) / 8, resident = sm_count() * 8;
+  // 16-byte loads of the logits (1) and of the bias (2)
+  const int vec = p.experts % 4 != 0 ? 0 : ((reinterpret_cast<uintptr_t>(p.logits) & 15) == 0 ? 1 : 0) |
+                                                 ((reinterpret_cast<uintptr_t>(p.bias) & 15) == 0 ? 2 : 0);
+  const int blocks = (p.tokens + 7) / 8, resident = sm_count() * 4;   // the CTAs that run at once
   launch_kernel(p.experts == 32 * PER ? moe_route_kernel<PER, true> : moe_route_kernel<PER, false>,
                 dim3(blocks < resident ? blocks : resident), dim3(256), 0, stream, p, group_lanes, vec);
   return check_cuda(cudaGetLastError(), "moe_route_kernel launch");
