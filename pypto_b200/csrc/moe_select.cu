@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) moe_route_any_kernel(const R
 // answer has a key of at least that (less the error): a handful of candidates instead of topk rounds over all experts.
 // They go to shared memory, one lane takes one of them and counts how many come before it.  If two candidates, or a
 // group that stays and one that goes, are closer than the error bound, the warp works the keys concerned out in 64 bits
-// and counts again; more than 32 candidates, too few available experts and infinite or NaN inputs go to route_token_f64.
+// and counts again; more than 32 candidates, too few available experts and infinite or NaN inputs go to route_lanes_f64.
 // The weights come from the chosen experts' logits with full 32-bit functions, whatever the keys went through.
 //
 // What bounds it is the number of instructions, 500 to 800 warp instructions a token (the 17 MB of logits of 16384 tokens
@@ -157,9 +157,11 @@ __global__ void __launch_bounds__(kRouteWarps * 32) moe_route_any_kernel(const R
 //
 // Error of a key: __expf is off by 2 + 1.173 |x| ulp of itself, which a sigmoid turns into at most s (1 - s) (2 + 1.173
 // |x|) 2^-23 < 0.8 * 2^-23; the sum and the approximate quotient add 3 ulp of s <= 1, adding the bias half an ulp of the
-// key: below 5e-7 + 2^-24 |key|.  Softmax: p (2 + 1.173 |x - max|) 2^-23 < 2.5 * 2^-23 for p <= exp(x - max), and the
-// sum's own error, p * 2^-20: below 1.3e-6 + 2^-24 |key|.  Two keys can be told apart beyond twice that: kTol...
-constexpr float kTolSigmoid = 1.1e-6f, kTolSoftmax = 2.7e-6f, kTolRel = 2.4e-7f;
+// key: below 5e-7 + 2^-24 |key|.  Softmax: expf is within 2 ulp of its rounded argument, p (2 + |x - max| / 2) 2^-23 <
+// 2.2 * 2^-23 for p <= exp(x - max); the sum takes up to 31 additions in a lane and five across, its reciprocal and the
+// product round once each, p * 38 * 2^-24: below 2.6e-6 + 2^-24 |key|.  Two keys can be told apart beyond twice that (the
+// last bits of kTolRel are the comparison's own rounding).
+constexpr float kTolSigmoid = 1.1e-6f, kTolSoftmax = 5.2e-6f, kTolRel = 2.4e-7f;
 
 // Floats as integers of the same order (no NaN), for the integer reductions of a warp.
 __device__ __forceinline__ int ordered_int(float v) {
