@@ -9,6 +9,7 @@ library's kernels.  There is no CPU path: CPU tensors raise.
 
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -23,8 +24,12 @@ if hasattr(torch, "float8_e8m0fnu"):
     _DT[torch.float8_e8m0fnu] = _lib.PTO_UINT8          # E8M0 scale codes travel as bytes
 
 FP8 = torch.float8_e4m3fn
+_WIDE = (torch.bfloat16, torch.float32)
 
 _scratch: dict[tuple[int, int], torch.Tensor] = {}
+
+
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def dtype_code(dt: torch.dtype) -> int:
@@ -53,17 +58,40 @@ def _need_cuda(*tensors: torch.Tensor) -> torch.device:
 def _stream_ptr(dev: torch.device) -> int:
     """torch's current stream on ``dev`` (a tensor's device).  The raw handle: building the Stream object around it
     takes 2 us, as long as a small kernel."""
-    return torch._C._cuda_getCurrentRawStream(dev.index if dev.index is not None else torch.cuda.current_device())
+    return _raw_stream(dev.index if dev.index is not None else torch.cuda.current_device())
 
 
-def _launch(dev: torch.device, entry, *args) -> None:
-    """One call into the library with ``dev`` as the current device (which it nearly always is: the context manager
+def _device_index(tensors) -> int:
+    """The checks of ``_need_cuda`` for operators whose calls are a few microseconds: the index of the one CUDA device
+    that all tensors lie on."""
+    index = None
+    for t in tensors:
+        if not isinstance(t, torch.Tensor) or not t.is_cuda or not t.is_contiguous():
+            _need_cuda(t)                                   # says which of these it is
+        i = t.get_device()
+        if i != index:
+            if index is not None:
+                raise ValueError("tensors are on different devices")
+            index = i
+    return index
+
+
+def _launch(index: int, entry, *args) -> None:
+    """One call into the library with CUDA device ``index`` current (which it nearly always is: the context manager
     costs 1.4 us)."""
-    if torch._C._cuda_getDevice() == dev.index:
-        _lib.check(entry(*args))
+    if torch._C._cuda_getDevice() == index:
+        status = entry(*args)
     else:
-        with torch.cuda.device(dev):
-            _lib.check(entry(*args))
+        with torch.cuda.device(index):
+            status = entry(*args)
+    if status:
+        _lib.check(status)
+
+
+def _error_word(index: int, stream: int) -> int:
+    """Address of the error word of a device and stream: the start of its scratch buffer."""
+    buf = _scratch.get((index, stream))
+    return buf.data_ptr() if buf is not None else scratch(torch.device("cuda", index), 256).data_ptr()
 
 
 def scratch(dev: torch.device, nbytes: int) -> torch.Tensor:
@@ -246,7 +274,12 @@ def linear_fp8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale:
     """out[m, n] = (acc +) x @ W with FP8 rows x (e4m3 [m, k], x_scale fp32 [m, ceil(k/128)], as ``quantize_rows`` and
     its fused forms write them) and a weight w e4m3 [n, k] with one fp32 scale per 128 x 128 block (w_scale
     [ceil(n/128), ceil(k/128)]).  out bf16 or fp32 (``out_dtype`` when it is not given); acc fp32 [m, n], may be out."""
-    dev = _need_cuda(*[t for t in (x, x_scale, w, w_scale, acc, out) if t is not None])
+    tensors = [x, x_scale, w, w_scale]
+    if acc is not None:
+        tensors.append(acc)
+    if out is not None:
+        tensors.append(out)
+    index = _device_index(tensors)
     if x.dtype != FP8 or w.dtype != FP8 or x.dim() != 2 or w.dim() != 2:
         raise TypeError("linear_fp8: x and w must be 2-D float8_e4m3fn tensors")
     m, k = x.shape
@@ -256,19 +289,20 @@ def linear_fp8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale:
     kb = (k + 127) // 128
     if x_scale.dtype != torch.float32 or w_scale.dtype != torch.float32:
         raise TypeError("linear_fp8: scales must be fp32")
-    if tuple(x_scale.shape) != (m, kb) or tuple(w_scale.shape) != ((n + 127) // 128, kb):
+    if x_scale.shape != (m, kb) or w_scale.shape != ((n + 127) // 128, kb):
         raise ValueError(f"linear_fp8: scales must be [{m}, {kb}] and [{(n + 127) // 128}, {kb}]")
     if out is None:
-        if out_dtype not in (torch.bfloat16, torch.float32):
+        if out_dtype not in _WIDE:
             raise TypeError("linear_fp8: out is bf16 or fp32")
-        out = torch.empty(m, n, dtype=out_dtype, device=dev)
-    elif out.dtype not in (torch.bfloat16, torch.float32) or tuple(out.shape) != (m, n):
+        out = torch.empty(m, n, dtype=out_dtype, device=x.device)
+    elif out.dtype not in _WIDE or out.shape != (m, n):
         raise ValueError("linear_fp8: out must be a bf16 or fp32 [m, n] tensor")
-    if acc is not None and (acc.dtype != torch.float32 or tuple(acc.shape) != (m, n)):
+    if acc is not None and (acc.dtype != torch.float32 or acc.shape != (m, n)):
         raise ValueError("linear_fp8: acc must be fp32 [m, n]")
-    _launch(dev, _lib.load().pto_linear_fp8, x.data_ptr(), x_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(),
-            acc.data_ptr() if acc is not None else None, out.data_ptr(), dtype_code(out.dtype), m, n, k, _err_ptr(dev),
-            _stream_ptr(dev))
+    stream = _raw_stream(index)
+    _launch(index, _lib.load().pto_linear_fp8, x.data_ptr(), x_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(),
+            acc.data_ptr() if acc is not None else None, out.data_ptr(), _DT[out.dtype], m, n, k,
+            _error_word(index, stream), stream)
     return out
 
 
@@ -341,44 +375,45 @@ def rms_norm(x: torch.Tensor, gamma: torch.Tensor | None, eps: float, out_dtype:
     return out
 
 
-_WIDE = (torch.bfloat16, torch.float32)
-
-
 def _norm_call(x, residual, gamma, eps, out_dtype, residual_out, quantize: bool, name: str):
     tensors = [x]
-    for t, what in ((residual, "residual"), (residual_out, "residual_out")):
-        if t is not None:
-            tensors.append(t)
-            if t.dtype not in _WIDE or t.shape != x.shape:
-                raise ValueError(f"{name}: {what} must be bf16 or fp32 with the shape of x")
+    if residual is not None:
+        tensors.append(residual)
+    if residual_out is not None:
+        tensors.append(residual_out)
     if gamma is not None:
         tensors.append(gamma)
-    dev = _need_cuda(*tensors)
+    index = _device_index(tensors)
     shape = x.shape
     if len(shape) < 1 or shape[-1] < 1 or x.dtype not in _WIDE:
         raise TypeError(f"{name}: x must be bf16 or fp32 [..., hidden]")
+    if residual is not None and (residual.dtype not in _WIDE or residual.shape != shape):
+        raise ValueError(f"{name}: residual must be bf16 or fp32 with the shape of x")
+    if residual_out is None:
+        residual_out = residual
+    elif residual_out.dtype not in _WIDE or residual_out.shape != shape:
+        raise ValueError(f"{name}: residual_out must be bf16 or fp32 with the shape of x")
+    elif residual is not None and residual.dtype != residual_out.dtype:
+        raise ValueError(f"{name}: residual and residual_out must have one dtype")
     hidden = shape[-1]
     if gamma is not None and (gamma.dtype != torch.float32 or gamma.numel() != hidden):
         raise ValueError(f"{name}: gamma must be fp32 with hidden elements")
     if out_dtype is not None and out_dtype not in _WIDE:
         raise TypeError(f"{name}: the normed rows are bf16 or fp32")
-    if residual_out is None:
-        residual_out = residual
-    elif residual is not None and residual.dtype != residual_out.dtype:
-        raise ValueError(f"{name}: residual and residual_out must have one dtype")
+    dev = x.device
     out = q = scale = None
     if out_dtype is not None:
-        out = torch.empty(shape, dtype=out_dtype, device=dev)
+        out = torch.empty(*shape, dtype=out_dtype, device=dev)      # sizes one by one: a tuple takes twice as long
     if quantize:
-        q = torch.empty(shape, dtype=FP8, device=dev)
-        scale = torch.empty((*shape[:-1], (hidden + 127) // 128), dtype=torch.float32, device=dev)
-    _launch(dev, _lib.load().pto_add_rms_norm,
+        q = torch.empty(*shape, dtype=FP8, device=dev)
+        scale = torch.empty(*shape[:-1], (hidden + 127) // 128, dtype=torch.float32, device=dev)
+    _launch(index, _lib.load().pto_add_rms_norm,
             x.data_ptr(), _DT[x.dtype], None if residual is None else residual.data_ptr(),
             None if residual_out is None else residual_out.data_ptr(),
             _lib.PTO_FP32 if residual_out is None else _DT[residual_out.dtype],
             None if gamma is None else gamma.data_ptr(), None if out is None else out.data_ptr(),
-            _lib.PTO_BF16 if out is None else _DT[out_dtype], q.data_ptr() if quantize else None,
-            scale.data_ptr() if quantize else None, x.numel() // hidden, hidden, float(eps), _stream_ptr(dev))
+            _lib.PTO_BF16 if out is None else _DT[out_dtype], None if q is None else q.data_ptr(),
+            None if q is None else scale.data_ptr(), x.numel() // hidden, hidden, eps, _raw_stream(index))
     return out, q, scale
 
 
@@ -455,15 +490,15 @@ def swiglu_act(gate_up: torch.Tensor) -> torch.Tensor:
 def swiglu_quantize(gate_up: torch.Tensor):
     """silu(gate) * up of gate_up bf16/fp32 [rows, 2*inter] (gate columns first) as FP8 rows: (q e4m3 [rows, inter],
     scale fp32 [rows, ceil(inter/128)])."""
-    dev = _need_cuda(gate_up)
-    if gate_up.dim() != 2 or gate_up.shape[1] < 2 or gate_up.shape[1] % 2 or \
-            gate_up.dtype not in (torch.bfloat16, torch.float32):
+    index = _device_index((gate_up,))
+    shape = gate_up.shape
+    if len(shape) != 2 or shape[1] < 2 or shape[1] % 2 or gate_up.dtype not in _WIDE:
         raise ValueError("swiglu_quantize: gate_up must be bf16/fp32 [rows, 2*inter]")
-    rows, inter = gate_up.shape[0], gate_up.shape[1] // 2
+    rows, inter, dev = shape[0], shape[1] // 2, gate_up.device
     q = torch.empty(rows, inter, dtype=FP8, device=dev)
     scale = torch.empty(rows, (inter + 127) // 128, dtype=torch.float32, device=dev)
-    _launch(dev, _lib.load().pto_swiglu_quantize, gate_up.data_ptr(), dtype_code(gate_up.dtype), q.data_ptr(),
-            scale.data_ptr(), rows, inter, _stream_ptr(dev))
+    _launch(index, _lib.load().pto_swiglu_quantize, gate_up.data_ptr(), _DT[gate_up.dtype], q.data_ptr(),
+            scale.data_ptr(), rows, inter, _raw_stream(index))
     return q, scale
 
 
@@ -492,6 +527,7 @@ def moe_topk(scores: torch.Tensor, bias: torch.Tensor | None, topk: int, is_logi
 SCORING = {"sigmoid": 0, "softmax": 1}      # PTO_SCORE_*
 
 
+@functools.lru_cache(maxsize=256)
 def check_routing(experts: int, topk: int, scoring: str, n_group: int, topk_group: int, group_top: int) -> None:
     """Raises ValueError for a routing that ``moe_route`` does not compute."""
     if scoring not in SCORING:
@@ -517,18 +553,20 @@ def moe_route(logits: torch.Tensor, topk: int, *, bias: torch.Tensor | None = No
     the topk_group groups with the largest sum of their best ``group_top`` keys stay; the topk experts by key are listed
     in descending order, ties to the lower id.  Weight = score, divided by the sum of the chosen scores if
     ``renormalize``, times ``route_scale``.  A bias of -inf takes an expert out."""
-    dev = _need_cuda(logits) if bias is None else _need_cuda(logits, bias)
-    if logits.dtype not in (torch.float32, torch.bfloat16) or logits.dim() != 2:
+    index = _device_index((logits,) if bias is None else (logits, bias))
+    shape = logits.shape
+    if logits.dtype not in _WIDE or len(shape) != 2:
         raise TypeError("moe_route: logits must be fp32 or bf16 [tokens, experts]")
-    t, e = logits.shape
+    t, e = shape
     check_routing(e, topk, scoring, n_group, topk_group, group_top)
     if bias is not None and (bias.dtype != torch.float32 or bias.numel() != e):
         raise ValueError("moe_route: bias must be fp32 [experts]")
+    dev = logits.device
     idx = torch.empty(t, topk, dtype=torch.int32, device=dev)
     w = torch.empty(t, topk, dtype=torch.float32, device=dev)
-    _launch(dev, _lib.load().pto_moe_route, logits.data_ptr(), dtype_code(logits.dtype),
+    _launch(index, _lib.load().pto_moe_route, logits.data_ptr(), _DT[logits.dtype],
             bias.data_ptr() if bias is not None else None, SCORING[scoring], t, e, n_group, topk_group, group_top, topk,
-            1 if renormalize else 0, float(route_scale), idx.data_ptr(), w.data_ptr(), _stream_ptr(dev))
+            1 if renormalize else 0, route_scale, idx.data_ptr(), w.data_ptr(), _raw_stream(index))
     return idx, w
 
 
