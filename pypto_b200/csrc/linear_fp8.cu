@@ -6,7 +6,7 @@
 //
 // It is the dense counterpart of the grouped expert GEMM (the numerics of the reference's block-scaled golden,
 // tests/st/runtime/ops/test_matmul_mx.py:119-131, with fp32 scales per 128).  Products and sums are fp32; out is rounded
-// once.  The order of additions depends on the sizes alone: equal calls give equal bits.
+// once.  The order of additions depends on sizes and alignment alone: equal calls give equal bits.
 #include "common.cuh"
 #include "kernels.h"
 #include "pair.cuh"
@@ -739,14 +739,16 @@ int pair_launch(const LinFp8Params& p, cudaStream_t stream) {
   return check_cuda(cudaGetLastError(), "linear_fp8_pair_kernel launch");
 }
 
-// Which tile for more than 64 tokens: the time of either in nanoseconds, from a start-up, a cost per round of tiles and a
-// cost per K block that fit the measurements (us, narrow / pair): m = 256, n = k = 4096 12.4 / 20.7;  512, 4096, 4096
-// 18.7 / 19.4;  1024, 1024, 4096 12.1 / 16.9;  777, 1000, 2000 9.4 / 11.6;  1024, 4096, 4096 36.3 / 17.7;
-// 256, 28672, 4096 71.3 / 34.4.  Up to 64 tokens the narrow tile wins throughout (64, 28672, 4096: 25.4 / 30.3).
+// Which tile: the time of each in nanoseconds, from a start-up, a cost per round of tiles and a cost per K block that fit the
+// measurements (us; 128-token / 32-token narrow tiles / pair): 256 x 4096 x 4096 12.4 / 16.4 / 20.7;  512 x 4096 x 4096
+// 18.7 / - / 19.4;  1024 x 1024 x 4096 12.1 / - / 16.9;  777 x 1000 x 2000 9.4 / 11.7 / 11.6;  300 x 640 x 4096 8.6 / 7.7 / -;
+// 150 x 512 x 512 7.8 / 4.4 / -;  1024 x 4096 x 4096 36.3 / - / 17.7;  256 x 28672 x 4096 71.3 / - / 34.4.  A pair is not
+// asked up to 64 tokens (64 x 28672 x 4096: 25.4 narrow, 30.3 pair).
 long long narrow_time(const LinFp8Params& p, int bn, int split) {
   const long long ctas = static_cast<long long>((p.m + bn - 1) / bn) * ((p.n + 127) / 128) * split;
   const long long slots = static_cast<long long>(sm_count()) * (bn <= 64 ? 2 : 1), rounds = (ctas + slots - 1) / slots;
-  return 2000 + rounds * (3000 + 450ll * ((p.kblocks + split - 1) / split)) + (split > 1 ? 1000 : 0);
+  const long long start = bn <= 32 ? 1800 : (bn <= 64 ? 2400 : 3000);
+  return 2000 + rounds * (start + 450ll * ((p.kblocks + split - 1) / split)) + (split > 1 ? (bn <= 64 ? 300 : 1000) : 0);
 }
 long long pair_time(const LinFp8Params& p) {
   const long long tiles = static_cast<long long>((p.m + 255) / 256) * ((p.n + 255) / 256), pairs = sm_count() / 2;
@@ -770,8 +772,14 @@ int linear_fp8_launch(const void* x, const float* x_scale, const void* w, const 
   p.vec = n % 4 == 0 && ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(acc)) & 15) == 0;
   const bool tma = k % 16 == 0 && ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w)) & 15) == 0;
   if (tma) {
-    const int bn = m <= 16 ? 16 : (m <= 32 ? 32 : (m <= 64 ? 64 : 128));
-    const int split = narrow_split(p, bn);
+    int bn = m <= 16 ? 16 : (m <= 32 ? 32 : (m <= 64 ? 64 : 128)), split = narrow_split(p, bn);
+    if (m > 32) {       // more and smaller tiles where the problem is small
+      const int split32 = narrow_split(p, 32);
+      if (split32 && (!split || narrow_time(p, 32, split32) < narrow_time(p, bn, split))) {
+        bn = 32;
+        split = split32;
+      }
+    }
     if (split == 0 || (m > 64 && pair_time(p) < narrow_time(p, bn, split))) return pair_launch(p, stream);
     switch (bn) {
       case 16: return narrow_launch<16>(p, split, stream);

@@ -217,7 +217,10 @@ def test_swiglu_quantize_odd_values():
 LINEAR_SIZES = [(1, 1, 16), (1, 128, 128), (1, 4096, 1024), (2, 130, 144), (8, 640, 2064), (17, 257, 2000), (31, 1000, 512),
                 (64, 512, 512), (65, 384, 1040), (100, 2048, 7168), (128, 128, 14336), (200, 1000, 2000), (257, 512, 400),
                 (300, 640, 4096), (513, 1152, 128), (777, 1000, 2000), (1024, 4096, 1024), (1500, 2200, 528),
-                (2049, 1025, 384), (5, 7, 5), (130, 129, 17), (70, 200, 333)]
+                (2049, 1025, 384), (5, 7, 5), (130, 129, 17), (70, 200, 333),
+                # the tile of 64 tokens, unsplit and split by eight; of 128, split by four and unsplit; pairs with few tokens
+                (64, 28672, 256), (50, 4096, 7168), (128, 4096, 4096), (512, 4096, 2048), (256, 28672, 528), (150, 512, 512),
+                (40, 520, 4112)]
 
 
 @pytest.mark.parametrize("m, n, k", LINEAR_SIZES)
