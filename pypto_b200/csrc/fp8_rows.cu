@@ -91,7 +91,10 @@ __global__ void __launch_bounds__(kRowThreads) add_rms_norm_any_kernel(const Add
 
 // Rows of any size and alignment up to 16384: a warp takes whole groups of 128 columns, E neighbouring elements to a lane
 // (two where sizes and addresses are even), and keeps its V groups of the row in registers between the two passes.
-// Bound by the number of two- and four-byte accesses: 3133 x 5003 bf16 with FP8 rows 62 us, 3133 x 5002 33 us.
+// All loads, gamma's too, are issued before the first sum, and the groups' maxima are reduced side by side: a warp's groups
+// one after the other cost half as much again (3133 x 5003 62 us, 1000 x 16383 112).  Bound by the number of two- and
+// four-byte accesses: bf16 with FP8 rows, 3133 x 5003 40 us, 3133 x 5002 32 us, 1000 x 16383 49 us.
+// Rows staged through shared memory with 16-byte copies gave 57 us at 3133 x 5003 and x 5002 alike.
 template <typename T, int E>
 struct RawN;
 template <>
@@ -141,9 +144,10 @@ __device__ __forceinline__ void st_codes(uint8_t* q, int left, const float (&y)[
     }
 }
 
+constexpr int kOddThreads = 512;
 template <typename TX, typename TR, int E, int V>
-__global__ void __launch_bounds__(kRowThreads) add_rms_norm_odd_kernel(const AddNormParams p) {
-  __shared__ float red[kRowThreads / 32];
+__global__ void __launch_bounds__(kOddThreads) add_rms_norm_odd_kernel(const AddNormParams p) {
+  __shared__ float red[kOddThreads / 32];
   pdl_launch_dependents();
   pdl_wait();
   const size_t base = static_cast<size_t>(blockIdx.x) * p.hidden;
@@ -160,6 +164,14 @@ __global__ void __launch_bounds__(kRowThreads) add_rms_norm_odd_kernel(const Add
       const int c = min((v * warps + warp) * kQuantGroup + (j * 32 + lane) * E, p.hidden - E);
       xr[v][j].load(x + c);
       if (r) rr[v][j].load(r + c);
+    }
+  float gm[V][4];
+#pragma unroll
+  for (int v = 0; v < V; ++v)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int c = (v * warps + warp) * kQuantGroup + (i / E * 32 + lane) * E + i % E;
+      gm[v][i] = p.gamma ? __ldg(p.gamma + min(c, p.hidden - 1)) : 1.f;
     }
   float h[V][4], ss = 0.f;
 #pragma unroll
@@ -180,28 +192,38 @@ __global__ void __launch_bounds__(kRowThreads) add_rms_norm_odd_kernel(const Add
   __syncthreads();
   ss = warp_sum(lane < warps ? red[lane] : 0.f);
   const float inv = rsqrtf(ss / static_cast<float>(p.hidden) + p.eps);
+  float amax[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    const int g = v * warps + warp, c0 = g * kQuantGroup + lane * E;
-    if (g >= p.groups) break;
-    float y[4], amax = 0.f;
+    amax[v] = 0.f;
 #pragma unroll
-    for (int j = 0; j < 4 / E; ++j) {
-      const int c = c0 + j * 32 * E;
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        y[j * E + e] = h[v][j * E + e] * inv * (p.gamma && c < p.hidden ? __ldg(p.gamma + c + e) : 1.f);
-        amax = fmaxf(amax, fabsf(y[j * E + e]));
-      }
-      if (p.out && c < p.hidden) {
-        if (p.out_bf16) st_n<E>(static_cast<__nv_bfloat16*>(p.out) + base + c, &y[j * E]);
-        else st_n<E>(static_cast<float*>(p.out) + base + c, &y[j * E]);
-      }
+    for (int i = 0; i < 4; ++i) {
+      h[v][i] = h[v][i] * inv * gm[v][i];
+      amax[v] = fmaxf(amax[v], fabsf(h[v][i]));
     }
-    if (p.q) {
-      const float s = e4m3_group_scale_fast(warp_max(amax));
-      st_codes<E>(p.q + base + c0, p.hidden - c0, y, s);
-      if (lane == 0) p.scale[static_cast<size_t>(blockIdx.x) * p.groups + g] = s;
+  }
+  if (p.out)
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+#pragma unroll
+      for (int j = 0; j < 4 / E; ++j) {
+        const int c = (v * warps + warp) * kQuantGroup + (j * 32 + lane) * E;
+        if (c < p.hidden) {
+          if (p.out_bf16) st_n<E>(static_cast<__nv_bfloat16*>(p.out) + base + c, &h[v][j * E]);
+          else st_n<E>(static_cast<float*>(p.out) + base + c, &h[v][j * E]);
+        }
+      }
+  if (p.q) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+      for (int v = 0; v < V; ++v) amax[v] = fmaxf(amax[v], __shfl_xor_sync(0xffffffffu, amax[v], o));
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int g = v * warps + warp, c0 = g * kQuantGroup + lane * E;
+      const float s = e4m3_group_scale_fast(amax[v]);
+      st_codes<E>(p.q + base + c0, p.hidden - c0, h[v], s);
+      if (lane == 0 && g < p.groups) p.scale[static_cast<size_t>(blockIdx.x) * p.groups + g] = s;
     }
   }
 }
@@ -469,13 +491,18 @@ int add_norm_units(const AddNormParams& p, long long rows, int threads, cudaStre
 
 template <typename TX, typename TR, int E>
 int add_norm_odd(const AddNormParams& p, long long rows, cudaStream_t stream) {
-  const dim3 grid(static_cast<unsigned>(rows)), block(32 * (p.groups < kRowThreads / 32 ? p.groups : kRowThreads / 32));
-  const int v = (p.groups + kRowThreads / 32 - 1) / (kRowThreads / 32);
+  // Eight warps, while that leaves a warp no more than six groups, for pairs (3133 x 5002 32 us, with sixteen 37); sixteen
+  // for single elements, which need more loads in flight (3133 x 5003 40 us, with eight 44), and for longer rows.
+  const int most = E == 2 && p.groups <= 48 ? 8 : kOddThreads / 32;
+  const int v = (p.groups + most - 1) / most, warps = (p.groups + v - 1) / v;
+  const dim3 grid(static_cast<unsigned>(rows)), block(32 * warps);
   if (v <= 1) launch_kernel(add_rms_norm_odd_kernel<TX, TR, E, 1>, grid, block, 0, stream, p);
   else if (v <= 2) launch_kernel(add_rms_norm_odd_kernel<TX, TR, E, 2>, grid, block, 0, stream, p);
+  else if (v <= 3) launch_kernel(add_rms_norm_odd_kernel<TX, TR, E, 3>, grid, block, 0, stream, p);
   else if (v <= 4) launch_kernel(add_rms_norm_odd_kernel<TX, TR, E, 4>, grid, block, 0, stream, p);
-  else if (v <= 8) launch_kernel(add_rms_norm_odd_kernel<TX, TR, E, 8>, grid, block, 0, stream, p);
-  else launch_kernel(add_rms_norm_odd_kernel<TX, TR, E, 16>, grid, block, 0, stream, p);
+  else if (v <= 5) launch_kernel(add_rms_norm_odd_kernel<TX, TR, E, 5>, grid, block, 0, stream, p);
+  else if (v <= 6) launch_kernel(add_rms_norm_odd_kernel<TX, TR, E, 6>, grid, block, 0, stream, p);
+  else launch_kernel(add_rms_norm_odd_kernel<TX, TR, E, 8>, grid, block, 0, stream, p);
   return check_cuda(cudaGetLastError(), "add_rms_norm_odd_kernel launch");
 }
 

@@ -59,7 +59,8 @@ def _norm_bound(hidden):
 
 
 NORM_SIZES = [(1, 1), (1, 4096), (3, 7), (5, 130), (2, 1000), (64, 7168), (33, 2048), (7, 128), (4, 1032), (300, 640),
-              (2, 16384), (3, 16392), (2, 20000), (1, 49152), (3, 5003), (2, 16383), (5, 2050), (2, 777), (4, 10222)]
+              (2, 16384), (3, 16392), (2, 20000), (1, 49152), (3, 5003), (2, 16383), (5, 2050), (2, 777), (4, 10222),
+              (3, 1030), (2, 8189), (2, 12001), (1, 6142)]
 
 
 @pytest.mark.parametrize("rows, hidden", NORM_SIZES)
