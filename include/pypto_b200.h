@@ -108,8 +108,8 @@ PTO_API int pto_worker_scratch(pto_worker* w, size_t min_bytes, uint64_t* dev_pt
 /* Registered callables (replaces Worker.register / Worker.run with a ChipCallable:
  * device_runner.py:651-656, worker.py:532-626).  `op_name` names a fused operator:
  * "paged_attention", "paged_gather", "rms_norm", "ffn_swiglu", "linear", "rope_kv_append", "scope3",
- * "decoder_layer", "matmul_mx", "add_rms_norm", "linear_fp8", "swiglu_quantize", "moe_route" (pto_op_list; tensor and scalar order beside each adapter in csrc/ops.cpp and
- * csrc/layer_ops.cpp). */
+ * "decoder_layer", "matmul_mx", "add_rms_norm", "linear_fp8", "swiglu_quantize", "moe_route" (pto_op_list;
+ * tensor and scalar order beside each adapter in csrc/ops.cpp and csrc/layer_ops.cpp). */
 PTO_API int pto_register_callable(pto_worker* w, const char* op_name, int32_t* cid);
 PTO_API int pto_unregister_callable(pto_worker* w, int32_t cid);
 PTO_API int pto_run(pto_worker* w, int32_t cid, const pto_task_args* args);

@@ -451,8 +451,9 @@ __global__ void __launch_bounds__(256, PER <= 8 ? 4 : 2) moe_route_kernel(const 
             above += (k4.x >= low) + (k4.y >= low) + (k4.z >= low) + (k4.w >= low);
           }
           const bool near = lane < n && above != rank + 1;
-          // logits and scores order alike as long as exp(x - max) is an ordinary number
-          if (by_logit && __any_sync(kAll, lane < n && xi - top < -80.f)) {
+          // Scores near the lowest 32-bit numbers lose the ratio that renormalising keeps, and no longer order like the
+          // logits: 64 bits.
+          if (__any_sync(kAll, lane < n && (p.softmax ? xi - top : xi) < -80.f)) {
             slow = true;
           } else if (__any_sync(kAll, near)) {
             const double total = p.softmax ? route_sum_f64(p, row, lane, top) : 1.0;

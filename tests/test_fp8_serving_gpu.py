@@ -360,6 +360,24 @@ def test_route_ties_and_borders(scoring):
 
 
 @pytest.mark.parametrize("scoring", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("depth", [79.0, 86.5, 95.0, 104.0, 300.0])
+def test_route_weights_of_the_lowest_scores(scoring, depth):
+    """Scores of e^-79 to e^-300 share the weight of a row in their own proportions."""
+    g = torch.Generator().manual_seed(5)
+    logits = torch.randn(20, 64, generator=g) - depth
+    bias = None
+    if scoring == "softmax":                                    # one expert has the mass; the bias keeps it out
+        logits[:, 63] = 0
+        bias = torch.zeros(64)
+        bias[63] = -math.inf
+    for kw in (dict(), dict(n_group=8, topk_group=4, group_top=2)):
+        _, w = _check_route(logits, 6, bias, scoring=scoring, **kw)
+        assert ((w.double().sum(1) - 1).abs() <= 10 * 2.0 ** -23).all()
+        _check_route(logits, 6, bias, scoring=scoring, renormalize=False, **kw)
+    _check_route(logits[:, 40:].contiguous(), 6, None if bias is None else bias[40:], scoring=scoring)      # no more experts than lanes
+
+
+@pytest.mark.parametrize("scoring", ["sigmoid", "softmax"])
 def test_route_masks_and_odd_values(scoring):
     g = torch.Generator().manual_seed(4)
     inf = math.inf
