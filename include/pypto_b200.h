@@ -269,7 +269,7 @@ PTO_API int pto_rms_norm_ex(const void* x, int x_dtype, const float* gamma, void
 /* Residual addition and RMSNorm in one pass over the rows, with an optional 8-bit output:
  *   h = x + residual (fp32; residual NULL: h = x);  y = h * rsqrt(mean(h^2) + eps) * gamma
  *   x bf16 or fp32 [rows, hidden]; residual and residual_out of one dtype, bf16 or fp32 [rows, hidden];
- *   residual_out (or NULL) receives h and may be `residual` itself; gamma fp32 [hidden] or NULL
+ *   residual_out (or NULL) receives h and may be `residual` itself, or x if of its dtype; gamma fp32 [hidden] or NULL
  *   out (or NULL) receives y in out_dtype; q / scale (both or neither) receive y as FP8 rows: e4m3
  *   [rows, hidden] with scale fp32 [rows, ceil(hidden / 128)] = max |y| / 448 over 128 columns (1 where that is 0),
  *   the operands of pto_linear_fp8 and pto_moe_expert_gemm.  One of out and q at least.  hidden up to 49152.

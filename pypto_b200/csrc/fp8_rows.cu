@@ -550,6 +550,13 @@ int add_rms_norm_launch(const void* x, int x_dtype, const void* residual, void* 
   PTO_REQUIRE(out || q, "add_rms_norm: neither out nor q is given");
   PTO_REQUIRE((q == nullptr) == (scale == nullptr), "add_rms_norm: FP8 rows need both q and scale");
   PTO_REQUIRE(x, "add_rms_norm: NULL tensor");
+  // in place on whole rows only: a row is read before any of it is written, but a shifted one may belong to another CTA
+  const size_t count = static_cast<size_t>(rows) * hidden, x_bytes = count * (x_dtype == PTO_BF16 ? 2 : 4);
+  const size_t res_bytes = count * (res_dtype == PTO_BF16 ? 2 : 4);
+  PTO_REQUIRE((residual_out == x && res_dtype == x_dtype) || !overlaps(residual_out, res_bytes, x, x_bytes),
+              "add_rms_norm: residual_out overlaps x");
+  PTO_REQUIRE(residual_out == residual || !overlaps(residual_out, res_bytes, residual, res_bytes),
+              "add_rms_norm: residual_out overlaps residual");
   AddNormParams p;
   p.x = x; p.residual = residual; p.residual_out = residual_out; p.gamma = gamma; p.out = out;
   p.q = static_cast<uint8_t*>(q); p.scale = scale;

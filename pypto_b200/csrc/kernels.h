@@ -85,6 +85,12 @@ int cast_zero_launch(const void* in, int in_dtype, void* out, int out_dtype, lon
                      size_t zero_bytes, cudaStream_t stream);
 int pack_weight_launch(const void* src, int src_dtype, void* dst, int k, int n, cudaStream_t stream);
 
+// Whether two byte ranges have a byte in common (NULL: no range).
+inline bool overlaps(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return a && b && x < y + b_bytes && y < x + a_bytes;
+}
+
 // fp8_rows.cu
 int add_rms_norm_launch(const void* x, int x_dtype, const void* residual, void* residual_out, int res_dtype,
                         const float* gamma, void* out, int out_dtype, void* q, float* scale, long long rows, int hidden,

@@ -59,7 +59,8 @@ __global__ void __launch_bounds__(256) linear_fp8_any_kernel(const LinFp8Params 
   __shared__ float xs[kAnyK][kAnyTile + 1], ws[kAnyK][kAnyTile + 1];
   pdl_launch_dependents();
   pdl_wait();
-  const int n0 = blockIdx.x * kAnyTile, m0 = blockIdx.y * kAnyTile;
+  const int n_tiles = (p.n + kAnyTile - 1) / kAnyTile, mt = static_cast<int>(blockIdx.x) / n_tiles;
+  const int n0 = (static_cast<int>(blockIdx.x) - mt * n_tiles) * kAnyTile, m0 = mt * kAnyTile;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   float acc[4][4] = {}, part[4][4] = {};
   for (int k0 = 0; k0 < p.k; k0 += kAnyK) {
@@ -765,6 +766,8 @@ int linear_fp8_launch(const void* x, const float* x_scale, const void* w, const 
   if (m == 0) return kOk;
   PTO_REQUIRE(x && x_scale && w && w_scale && out, "linear_fp8: NULL tensor");
   PTO_REQUIRE(!(acc && acc == out && out_dtype != PTO_FP32), "linear_fp8: only an fp32 out may be the tensor that is added");
+  const size_t outputs = static_cast<size_t>(m) * n;
+  PTO_REQUIRE(acc == out || !overlaps(out, outputs * (out_dtype == PTO_BF16 ? 2 : 4), acc, outputs * 4), "linear_fp8: out overlaps acc");
   LinFp8Params p;
   p.x = static_cast<const uint8_t*>(x); p.x_scale = x_scale; p.w = static_cast<const uint8_t*>(w); p.w_scale = w_scale;
   p.acc = acc; p.out = out; p.m = m; p.n = n; p.k = k; p.kblocks = (k + 127) / 128; p.out_bf16 = out_dtype == PTO_BF16;
@@ -788,9 +791,9 @@ int linear_fp8_launch(const void* x, const float* x_scale, const void* w, const 
       default: return narrow_launch<128>(p, split, stream);
     }
   }
-  PTO_REQUIRE((m + kAnyTile - 1) / kAnyTile <= 65535, "linear_fp8: too many rows");
-  launch_kernel(linear_fp8_any_kernel, dim3((n + kAnyTile - 1) / kAnyTile, (m + kAnyTile - 1) / kAnyTile), dim3(256), 0,
-                stream, p);
+  const long long tiles = ((m + kAnyTile - 1ll) / kAnyTile) * ((n + kAnyTile - 1ll) / kAnyTile);
+  PTO_REQUIRE(tiles < (1ll << 31), "linear_fp8: problem too large");
+  launch_kernel(linear_fp8_any_kernel, dim3(static_cast<unsigned>(tiles)), dim3(256), 0, stream, p);
   return check_cuda(cudaGetLastError(), "linear_fp8_any_kernel launch");
 }
 

@@ -83,6 +83,9 @@ class Fp8SwiGLUFFN:
         self.hidden, self.inter = self.w_gu.shape[1], self.w_gu.shape[0] // 2
         if self.w_gu.shape[0] % 2 or tuple(self.w_d.shape) != (self.hidden, self.inter):
             raise ValueError("Fp8SwiGLUFFN: weights must be [2*inter, hidden] and [hidden, inter]")
+        for w, scale in (w_gate_up, w_down):
+            if w.dtype != ops.FP8 or tuple(scale.shape) != tuple((n + 127) // 128 for n in w.shape):
+                raise ValueError("Fp8SwiGLUFFN: weights must be e4m3 with one scale per 128 x 128 block")
 
     @classmethod
     def from_float(cls, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, gamma: torch.Tensor, eps: float):

@@ -420,7 +420,8 @@ def _norm_call(x, residual, gamma, eps, out_dtype, residual_out, quantize: bool,
 def add_rms_norm(x: torch.Tensor, residual: torch.Tensor | None, gamma: torch.Tensor | None, eps: float,
                  out_dtype: torch.dtype = torch.bfloat16, *, residual_out: torch.Tensor | None = None) -> torch.Tensor:
     """RMSNorm of the rows of x + residual; the sum goes to ``residual_out``, by default into ``residual`` itself
-    (rounded to its dtype; the norm is taken of the fp32 sum).  ``residual`` None: the norm of x."""
+    (rounded to its dtype; the norm is taken of the fp32 sum), or over x of the same dtype; any other overlap is refused.
+    ``residual`` None: the norm of x."""
     if out_dtype is None:
         raise TypeError("add_rms_norm: the normed rows are bf16 or fp32")
     return _norm_call(x, residual, gamma, eps, out_dtype, residual_out, False, "add_rms_norm")[0]

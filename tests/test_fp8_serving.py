@@ -38,9 +38,12 @@ def _swiglu(x=P, dt=BF16, q=P, s=P, rows=4, inter=64):
     (_norm, dict(rows=1 << 31), "rows"), (_norm, dict(xdt=FP16), "x must"), (_norm, dict(rdt=FP16), "residual"),
     (_norm, dict(odt=FP16), "out"), (_norm, dict(out=None), "neither"), (_norm, dict(q=P), "both"),
     (_norm, dict(s=P), "both"), (_norm, dict(eps=-1.0), "eps"), (_norm, dict(eps=math.nan), "eps"), (_norm, dict(x=None), "NULL"),
+    (_norm, dict(x=8 * P, res_out=P + 64), "overlaps residual"), (_norm, dict(x=P + 1024 - 4, res_out=P, res=None), "overlaps x"),
+    (_norm, dict(res=None), "overlaps x"), (_norm, dict(x=P + 1024, res_out=P + 4, res=None), "overlaps x"),
     (_linear, dict(n=0), "positive"), (_linear, dict(k=0), "positive"), (_linear, dict(m=-1), "positive"),
     (_linear, dict(m=(1 << 30) + 1), "2^30"), (_linear, dict(odt=FP16), "out"), (_linear, dict(x=None), "NULL"), (_linear, dict(ws=None), "NULL"),
-    (_linear, dict(acc=P), "fp32 out"),
+    (_linear, dict(acc=P), "fp32 out"), (_linear, dict(acc=P + 4, odt=FP32), "overlaps acc"),
+    (_linear, dict(acc=P - 1024 + 4), "overlaps acc"), (_linear, dict(acc=P + 512 - 4), "overlaps acc"),
     (_swiglu, dict(dt=FP16), "gate_up"), (_swiglu, dict(inter=0), "sizes"), (_swiglu, dict(rows=-1), "sizes"),
     (_swiglu, dict(q=None), "NULL"),
     (_route, dict(dt=FP16), "logits"), (_route, dict(scoring=2), "scoring"), (_route, dict(experts=1025), "experts"),
@@ -90,6 +93,11 @@ def test_layer_objects_check_their_arguments():
     assert (back - w.t().double()).abs().le(2 ** -4 * w.t().double().abs() + 2.0 ** -10 * s.max().item() + 1e-6).all()
     with pytest.raises(ValueError):
         Fp8SwiGLUFFN((q, s), (q, s), torch.ones(200), 1e-6)
+    down, down_s = quantize_weight(torch.randn(150, 200, generator=g))
+    Fp8SwiGLUFFN((q, s), (down, down_s), torch.ones(200), 1e-6)
+    for bad in ((down, down_s[:, :1]), (down.float(), down_s)):
+        with pytest.raises(ValueError):
+            Fp8SwiGLUFFN((q, s), bad, torch.ones(200), 1e-6)
     with pytest.raises(ValueError):
         MoELayer.from_packed(torch.zeros(6, 128, dtype=torch.bfloat16), torch.zeros(6), dict(w_gu=torch.zeros(6, 256, 128)), None,
                              topk=2, router=Router(n_group=4, topk_group=2))

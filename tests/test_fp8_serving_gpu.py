@@ -149,6 +149,26 @@ def test_add_rms_norm_odd_values_and_alignment():
         _check_fp8_rows_of(b[2], b[0], b[1])
 
 
+@pytest.mark.parametrize("hidden", [256, 777, 1030, 7168, 20000])
+@pytest.mark.parametrize("dt", [BF16, FP32])
+def test_add_rms_norm_sum_written_over_x(hidden, dt):
+    from pypto_b200 import _lib
+    ops = _ops()
+    g = _gen(hidden)
+    x, res = _randn(g, 40, hidden).to(dt), _randn(g, 40, hidden).to(dt)
+    total = torch.empty_like(x)
+    want = ops.add_rms_norm(x, res, None, 1e-6, residual_out=total)
+    over, keep = x.clone(), res.clone()
+    assert torch.equal(ops.add_rms_norm(over, keep, None, 1e-6, residual_out=over), want)
+    assert torch.equal(over, total) and torch.equal(keep, res)
+    both = x.clone()                                            # x + x, in place
+    twice = ops.add_rms_norm(x, x.clone(), None, 1e-6)
+    assert torch.equal(ops.add_rms_norm(both, both, None, 1e-6), twice) and torch.equal(both, 2 * x)
+    flat = torch.zeros(41 * hidden, dtype=dt, device="cuda")
+    with pytest.raises(_lib.PtoError):
+        ops.add_rms_norm(flat[:40 * hidden].view(40, hidden), None, None, 1e-6, residual_out=flat[hidden:].view(40, hidden))
+
+
 def test_add_rms_norm_refusals():
     ops = _ops()
     x = torch.zeros(4, 256, dtype=BF16, device="cuda")
@@ -217,7 +237,7 @@ def test_swiglu_quantize_odd_values():
 
 LINEAR_SIZES = [(1, 1, 16), (1, 128, 128), (1, 4096, 1024), (2, 130, 144), (8, 640, 2064), (17, 257, 2000), (31, 1000, 512),
                 (64, 512, 512), (65, 384, 1040), (100, 2048, 7168), (128, 128, 14336), (200, 1000, 2000), (257, 512, 400),
-                (300, 640, 4096), (513, 1152, 128), (777, 1000, 2000), (1024, 4096, 1024), (1500, 2200, 528),
+                (300, 640, 4096), (4500, 3, 5), (513, 1152, 128), (777, 1000, 2000), (1024, 4096, 1024), (1500, 2200, 528),
                 (2049, 1025, 384), (5, 7, 5), (130, 129, 17), (70, 200, 333),
                 # the tile of 64 tokens, unsplit and split by eight; of 128, split by four and unsplit; pairs with few tokens
                 (64, 28672, 256), (50, 4096, 7168), (128, 4096, 4096), (512, 4096, 2048), (256, 28672, 528), (150, 512, 512),
@@ -266,6 +286,7 @@ def test_linear_fp8_known_answers(m, n, k):
 
 
 def test_linear_fp8_odd_values_alignment_and_refusals():
+    from pypto_b200 import _lib
     ops = _ops()
     g = _gen(9)
     m, n, k = 40, 200, 256
@@ -294,6 +315,9 @@ def test_linear_fp8_odd_values_alignment_and_refusals():
     got = ops.linear_fp8(x, sflat[1:].view(xs.shape), w, wflat[1:].view(ws.shape), out=oflat[1:].view(m, n))
     assert torch.equal(got, want.to(BF16))
     assert ops.linear_fp8(x[:0], xs[:0], w, ws).shape == (0, n)
+    stream = torch.zeros(m + 1, n, device="cuda")               # the sum one row off its own place
+    with pytest.raises(_lib.PtoError):
+        ops.linear_fp8(x, xs, w, ws, acc=stream[:m], out=stream[1:])
     for args, kw, err in [((x, xs[:, :1].contiguous(), w, ws), {}, ValueError), ((x, xs, w, ws[:1].contiguous()), {}, ValueError),
                           ((x.view(torch.uint8), xs, w, ws), {}, TypeError), ((x, xs.double(), w, ws), {}, TypeError),
                           ((x[:, :128].contiguous(), xs[:, :1].contiguous(), w, ws), {}, ValueError),
