@@ -149,8 +149,9 @@ __global__ void __launch_bounds__(kRouteWarps * 32) moe_route_any_kernel(const R
 // The weights come from the chosen experts' logits with full 32-bit functions, whatever the keys went through.
 //
 // What bounds it is the number of instructions, 500 to 800 warp instructions a token (the 17 MB of logits of 16384 tokens
-// are 2.7 us of memory).  Measured, 256 experts, top 8: 16384 tokens 20.4 us with 4 of 8 groups, 16.2 us without groups (63 us
-// with everything in 64 bits and a round over all experts per choice), 4096 tokens 7.0 us, one token 3.2 us.  Tried:
+// are 2.7 us of memory).  Measured, 256 experts, top 8: 16384 tokens 18.2 us with 4 of 8 groups (19.6 us when a close border
+// works out all keys in 64 bits, not only those that may be among a group's best), 16.0 us without groups (63 us with
+// everything in 64 bits and a round over all experts per choice), 4096 tokens 6.5 us, one token 3.1 us.  Tried:
 // putting close tokens off to the CTA's end (fewer registers, but 21-22 us: the late ones are a tail), five or six CTAs an
 // SM instead of four (spills, 23-28 us), eight or sixteen rounds of CTAs instead of one resident set (20.5 us, but 7.8-8.4
 // us at 4096 tokens).
@@ -386,11 +387,16 @@ __global__ void __launch_bounds__(256, PER <= 8 ? 4 : 2) moe_route_kernel(const 
         if (at <= ordered_int(-FLT_MAX)) {
           slow = true;                               // fewer groups with an available expert than stay
         } else if (!(lo - hi > 2.f * most) || lo < -1e29f || __popc(__ballot_sync(kAll, kept)) != p.topk_group * group_lanes) {
+          // only the keys that may be among the group's best, a lane's own one after the other: one or two of its PER
+          const float cut = two ? b2 : b1, from = cut - (tol_abs + kTolRel * fabsf(cut));
+          unsigned open = 0;
+#pragma unroll
+          for (int j = 0; j < PER; ++j) open |= static_cast<unsigned>(key[j] > -INFINITY && key[j] >= from) << j;
           const double total = p.softmax ? route_sum_f64(p, row, lane, top) : 1.0;
           double d1 = -INFINITY, d2 = -INFINITY;
 #pragma unroll 1
-          for (int e = e0; e < min(e0 + PER, p.experts); ++e) {
-            const double k = route_key_f64(p, row, e, top, total);
+          for (; open; open &= open - 1) {
+            const double k = route_key_f64(p, row, e0 + __ffs(open) - 1, top, total);
             d2 = fmax(d2, fmin(d1, k));
             d1 = fmax(d1, k);
           }
