@@ -63,9 +63,11 @@ def _stream_ptr(dev: torch.device) -> int:
 
 def _device_index(tensors) -> int:
     """The checks of ``_need_cuda`` for operators whose calls are a few microseconds: the index of the one CUDA device
-    that all tensors lie on."""
+    that all tensors lie on (None after the first: an argument that is not given)."""
     index = None
     for t in tensors:
+        if t is None and index is not None:
+            continue
         if not isinstance(t, torch.Tensor) or not t.is_cuda or not t.is_contiguous():
             _need_cuda(t)                                   # says which of these it is
         i = t.get_device()
@@ -376,14 +378,7 @@ def rms_norm(x: torch.Tensor, gamma: torch.Tensor | None, eps: float, out_dtype:
 
 
 def _norm_call(x, residual, gamma, eps, out_dtype, residual_out, quantize: bool, name: str):
-    tensors = [x]
-    if residual is not None:
-        tensors.append(residual)
-    if residual_out is not None:
-        tensors.append(residual_out)
-    if gamma is not None:
-        tensors.append(gamma)
-    index = _device_index(tensors)
+    index = _device_index((x, residual, residual_out, gamma))
     shape = x.shape
     if len(shape) < 1 or shape[-1] < 1 or x.dtype not in _WIDE:
         raise TypeError(f"{name}: x must be bf16 or fp32 [..., hidden]")
@@ -400,13 +395,13 @@ def _norm_call(x, residual, gamma, eps, out_dtype, residual_out, quantize: bool,
         raise ValueError(f"{name}: gamma must be fp32 with hidden elements")
     if out_dtype is not None and out_dtype not in _WIDE:
         raise TypeError(f"{name}: the normed rows are bf16 or fp32")
-    dev = x.device
     out = q = scale = None
     if out_dtype is not None:
-        out = torch.empty(*shape, dtype=out_dtype, device=dev)      # sizes one by one: a tuple takes twice as long
+        out = torch.empty_like(x, dtype=out_dtype)
     if quantize:
-        q = torch.empty(*shape, dtype=FP8, device=dev)
-        scale = torch.empty(*shape[:-1], (hidden + 127) // 128, dtype=torch.float32, device=dev)
+        q = torch.empty_like(x, dtype=FP8)
+        # sizes one by one: a tuple takes twice as long
+        scale = torch.empty(*shape[:-1], (hidden + 127) // 128, dtype=torch.float32, device=x.device)
     _launch(index, _lib.load().pto_add_rms_norm,
             x.data_ptr(), _DT[x.dtype], None if residual is None else residual.data_ptr(),
             None if residual_out is None else residual_out.data_ptr(),
@@ -554,7 +549,7 @@ def moe_route(logits: torch.Tensor, topk: int, *, bias: torch.Tensor | None = No
     the topk_group groups with the largest sum of their best ``group_top`` keys stay; the topk experts by key are listed
     in descending order, ties to the lower id.  Weight = score, divided by the sum of the chosen scores if
     ``renormalize``, times ``route_scale``.  A bias of -inf takes an expert out."""
-    index = _device_index((logits,) if bias is None else (logits, bias))
+    index = _device_index((logits, bias))
     shape = logits.shape
     if logits.dtype not in _WIDE or len(shape) != 2:
         raise TypeError("moe_route: logits must be fp32 or bf16 [tokens, experts]")
